@@ -1015,6 +1015,72 @@ int zshmc_uni2_sample(int kind, float* out, const float* a, const float* b,
                       int64_t n, int64_t inner, int a_bcast, int b_bcast,
                       uint64_t seed, uint32_t offset, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Linear output layers over many classes
+ * ------------------------------------------------------------------------ */
+/* element types of the operands below */
+#define ZSHMC_DTYPE_F32 0
+#define ZSHMC_DTYPE_BF16 1
+
+/* log_prob[n] = log Categorical(labels[n] | logits = x[n, :] . w[v, :] + bias[v])
+ * (distributions/univariate.py:496-548) with the classes taken in pieces: no
+ * [n_rows, n_classes] array exists at any time.
+ *   x [n_rows, n_features], w [n_classes, n_features]: `dtype`, rows ldx / ldw
+ *                  elements apart; bias [n_classes] float32 or NULL
+ *   labels         int64; has_ignore: rows labelled `ignore_label` get 0 and
+ *                  have no part in any gradient, whatever x holds there; any
+ *                  other label outside [0, n_classes) gives NaN
+ *   stats          [n_rows][2] float32 (maximum, sum of exponentials) for the
+ *                  gradient, 8-byte aligned, or NULL
+ *   workspace      16-byte aligned; its size from
+ *                  zshmc_class_log_prob_workspace with the SAME pointers and
+ *                  strides (gradient = 0 / 1 for the two calls), written to
+ *                  *n_bytes_host.
+ * float32 operands are multiplied as three bfloat16 planes each, with
+ * float32-level results; accumulation is float32. */
+int zshmc_class_log_prob_workspace(const void* x, const void* w,
+                                   int64_t n_rows, int64_t n_features,
+                                   int64_t n_classes, int64_t ldx, int64_t ldw,
+                                   int dtype, int gradient, int has_ignore,
+                                   int64_t* n_bytes_host);
+int zshmc_class_log_prob(const void* x, const void* w, const float* bias,
+                         const int64_t* labels, int64_t n_rows,
+                         int64_t n_features, int64_t n_classes, int64_t ldx,
+                         int64_t ldw, int dtype, int has_ignore,
+                         int64_t ignore_label, float* log_prob, float* stats,
+                         void* workspace, int64_t workspace_bytes,
+                         void* stream);
+/* The gradients of sum_n grad_log_prob[n] log_prob[n]: grad_x [n_rows,
+ * n_features] and grad_w [n_classes, n_features] dense, of `dtype`, grad_bias
+ * [n_classes] float32; any may be NULL.  `stats` from the forward call on the
+ * same operands. */
+int zshmc_class_log_prob_grad(
+    const void* x, const void* w, const float* bias, const int64_t* labels,
+    int64_t n_rows, int64_t n_features, int64_t n_classes, int64_t ldx,
+    int64_t ldw, int dtype, int has_ignore, int64_t ignore_label,
+    const float* stats, const float* grad_log_prob, void* grad_x, void* grad_w,
+    float* grad_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows as 8-bit integers with one scale each: scale[r] = max|x[r, :]| / 127
+ * (1 for a row of zeros, NaN for a row with an infinity or a NaN), values =
+ * rint(x / scale), to even; zeros in the columns from n_cols to `pitch`. */
+int zshmc_quantize_rows(const void* x, int64_t n_rows, int64_t n_cols,
+                        int64_t ldx, int dtype, int8_t* values, int64_t pitch,
+                        float* scale, void* stream);
+/* out[r, c] = values[r, c] * scale[r] */
+int zshmc_dequantize_rows(const int8_t* values, int64_t pitch,
+                          const float* scale, int64_t n_rows, int64_t n_cols,
+                          void* out, int64_t ldo, int dtype, void* stream);
+/* out[m, n] = (x_scale[m] w_scale[n]) sum_k x[m, k] w[n, k] + bias[n] with
+ * 8-bit x and w and an exact sum (n_features <= 131072); bias may be NULL.
+ * Rows are 16-byte aligned with pitches of whole 16 bytes and readable up to
+ * the next multiple of 16 columns, where x holds zeros. */
+int zshmc_int8_linear(const int8_t* x, int64_t x_pitch, const float* x_scale,
+                      const int8_t* w, int64_t w_pitch, const float* w_scale,
+                      const float* bias, int64_t n_rows, int64_t n_features,
+                      int64_t n_channels, void* out, int64_t ldo, int dtype,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,265 @@
+"""zs.linear_categorical_log_prob (csrc/class_logits.hip) against its plain
+form in 64 bits, with the element-wise bounds of helpers_class_logits."""
+import pytest
+import torch
+
+import zhusuan_amd as zs
+from helpers_class_logits import class_log_prob, problem, within
+
+pytestmark = pytest.mark.gpu
+BOTH = [torch.float32, torch.bfloat16]
+IGNORE = -100
+
+
+def run(w, X, y, b, g, ignore=None):
+    leaves = [t.detach().clone(memory_format=torch.preserve_format)
+              .requires_grad_() if t.is_contiguous() else
+              t.detach().requires_grad_() for t in (w, X, b) if t is not None]
+    lp = zs.linear_categorical_log_prob(
+        leaves[0], leaves[1], y, bias=leaves[2] if b is not None else None,
+        ignore_label=ignore)
+    return lp, torch.autograd.grad(lp, leaves, g)
+
+
+def check(w, X, y, b, g, ignore=None):
+    lp, grads = run(w, X, y, b, g, ignore)
+    (ref, refs), (tol, tols) = class_log_prob(w, X, y, b, ignore, g)
+    within(lp, ref, tol, 'log_prob')
+    for name, got, r, t in zip(('w', 'X', 'bias'), grads, refs, tols):
+        within(got, r, t, name)
+    return lp, grads
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+@pytest.mark.parametrize('N,D,V', [
+    (1, 1, 1), (1, 64, 128), (2, 7, 3), (5, 8, 257), (31, 64, 300),
+    (32, 130, 129), (33, 128, 500), (65, 200, 1000), (129, 72, 4099),
+    (100, 128, 12419), (300, 256, 40000), (1021, 784, 1237)])
+def test_log_prob_and_gradients(N, D, V, dtype):
+    for bias, ignore in ((False, None), (True, IGNORE)):
+        w, X, y, b, g = problem(N, D, V, dtype, N + D + V, bias, ignore)
+        check(w, X, y, b, g, ignore)
+
+
+@pytest.mark.parametrize('dtype,N,V', [(torch.bfloat16, 8192, 20000),
+                                       (torch.float32, 6001, 9001)])
+def test_several_pieces_of_the_vocabulary(dtype, N, V):
+    w, X, y, b, g = problem(N, 64, V, dtype, 3, True, IGNORE)
+    check(w, X, y, b, g, IGNORE)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_ignored_rows_may_hold_anything(dtype):
+    w, X, y, b, g = problem(70, 96, 333, dtype, 5, True, IGNORE)
+    clean = run(w, X, y, b, g, IGNORE)
+    X2 = X.clone()
+    X2[y == IGNORE] = float('nan')
+    X2[0] = float('inf')
+    g2 = g.clone()
+    g2[y == IGNORE] = float('nan')
+    lp, grads = run(w, X2, y, b, g2, IGNORE)
+    assert torch.equal(lp, clean[0])
+    for a, c in zip(grads, clean[1]):
+        assert torch.equal(a, c)
+    assert bool((lp[y == IGNORE] == 0).all())
+    assert bool((grads[1][y == IGNORE] == 0).all())
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_every_row_ignored(dtype):
+    w, X, y, b, g = problem(20, 64, 100, dtype, 6, True)
+    y = torch.full_like(y, 7)
+    lp, grads = run(w, X, y, b, g, ignore=7)
+    assert bool((lp == 0).all())
+    assert all(bool((t == 0).all()) for t in grads)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_masked_classes(dtype):
+    """A bias of -inf takes a class out: its probability and its gradients are
+    zero; a row whose label it is has -inf; float32's lowest does the same."""
+    w, X, y, b, g = problem(40, 64, 600, dtype, 7, True)
+    b[256:520] = -float('inf')          # whole tiles among them
+    b[3] = torch.finfo(torch.float32).min
+    y = (y % 200) + 4                   # labels that stay
+    lp, grads = check(w, X, y, b, g)
+    assert bool((grads[0][256:520] == 0).all())
+    assert bool((grads[2][256:520] == 0).all())
+    y2 = y.clone()
+    y2[5] = 300
+    lp2, _ = run(w, X, y2, b, g)
+    assert float(lp2[5]) == -float('inf')
+    keep = torch.arange(40, device='cuda') != 5
+    assert torch.equal(lp2[keep], lp[keep])
+    b[:] = -float('inf')                # nothing is left: no distribution
+    lp3 = zs.linear_categorical_log_prob(w, X, y, bias=b)
+    assert bool(lp3.isnan().all())
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_labels_outside(dtype):
+    w, X, y, b, g = problem(40, 64, 300, dtype, 8)
+    ref = run(w, X, y, b, g)
+    y2 = y.clone()
+    y2[3], y2[35] = 300, -1
+    lp, (gw, gx) = run(w, X, y2, b, g)
+    bad = torch.zeros(40, dtype=torch.bool, device='cuda')
+    bad[3] = bad[35] = True
+    assert torch.equal(lp.isnan(), bad)
+    assert torch.equal(gx.isnan().all(1), bad)
+    assert torch.equal(lp[~bad], ref[0][~bad])
+    assert torch.equal(gx[~bad], ref[1][1][~bad])
+    assert bool(gw.isnan().all())
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_nonfinite_rows_stay_their_own(dtype):
+    w, X, y, b, g = problem(34, 64, 300, dtype, 9)
+    ref = run(w, X, y, b, g)
+    X2 = X.clone()
+    X2[2, 5] = float('nan')
+    lp, (gw, gx) = run(w, X2, y, b, g)
+    bad = torch.zeros(34, dtype=torch.bool, device='cuda')
+    bad[2] = True
+    assert torch.equal(lp.isnan(), bad) and torch.equal(lp[~bad], ref[0][~bad])
+    assert torch.equal(gx[~bad], ref[1][1][~bad])
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_strides_alignment_and_shapes(dtype):
+    w, X, y, b, g = problem(60, 96, 410, dtype, 10, True)
+    ref = run(w, X, y, b, g)
+
+    def same(w_, X_, y_, b_):
+        lp, grads = run(w_, X_, y_, b_, g.reshape(y_.shape))
+        assert torch.equal(lp.reshape(-1), ref[0])
+        for a, c in zip(grads, ref[1]):
+            assert torch.equal(a.reshape(c.shape), c)
+    wide = torch.full((60, 250), float('nan'), device='cuda', dtype=dtype)
+    for off in (0, 1, 8, 77):           # rows inside a wider buffer, NaN around
+        wide[:] = float('nan')
+        wide[:, off:off + 96] = X
+        same(w, wide[:, off:off + 96], y, b)
+    ww = torch.full((2, 410, 99), float('nan'), device='cuda', dtype=dtype)
+    ww[1, :, 3:] = w
+    same(ww[1, :, 3:], X, y, b)
+    same(w.t().contiguous().t(), X.t().contiguous().t(), y.int(), b)
+    same(w, X.reshape(5, 12, 96), y.reshape(5, 12), b)
+    yy = torch.stack([y, y], 1)
+    bb = torch.stack([b, b], 1)
+    same(w, X, yy[:, 0], bb[:, 1])
+    # one row used for all: the gradient of the shared row is the sum
+    one = X[:1].detach().clone().requires_grad_()
+    lp = zs.linear_categorical_log_prob(w, one.expand(60, 96), y, bias=b)
+    gx, = torch.autograd.grad(lp, one, g)
+    (_, refs), (_, tols) = class_log_prob(w, X[:1].expand(60, 96), y, b, None,
+                                          g)
+    # (torch adds the 60 rows in their own type)
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    within(gx[0], refs[1].sum(0),
+           tols[1].sum(0) + 60 * half * refs[1].abs().sum(0), 'shared row')
+
+
+def test_bias_of_the_operands_type_and_partial_gradients():
+    w, X, y, b, g = problem(33, 64, 200, torch.bfloat16, 11, True)
+    bh = b.bfloat16().requires_grad_()
+    lp = zs.linear_categorical_log_prob(w, X, y, bias=bh)
+    gb, = torch.autograd.grad(lp, bh, g)
+    assert gb.dtype == torch.bfloat16
+    full = run(w, X, y, bh.detach().float(), g)
+    assert torch.equal(lp, full[0]) and torch.equal(gb, full[1][2].bfloat16())
+    for leaf, k in ((w, 0), (X, 1)):    # one gradient alone
+        t = leaf.clone().requires_grad_()
+        args = (t, X) if k == 0 else (w, t)
+        lp = zs.linear_categorical_log_prob(*args, y, bias=bh.detach())
+        got, = torch.autograd.grad(lp, t, g)
+        assert torch.equal(got, full[1][k])
+    with torch.no_grad():
+        assert torch.equal(zs.linear_categorical_log_prob(w, X, y, bias=bh),
+                           lp)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_empty(dtype):
+    w, X, y, b, g = problem(4, 33, 101, dtype, 12, True)
+    lp, grads = run(w, X[:0], y[:0], b, g[:0])
+    assert lp.shape == (0,) and grads[1].shape == (0, 33)
+    assert bool((grads[0] == 0).all()) and bool((grads[2] == 0).all())
+
+
+def test_gradients_against_differences():
+    """(f(x + h) - f(x - h)) / 2h in float32: off by 2 E / 2h for a function
+    known to E, and by h^2 / 6 times the third derivative, at most |w_d|^3 (for
+    X; third cumulants of a variable within +-a are below 2 a^3, those of an
+    indicator below 1)."""
+    w, X, y, b, g = problem(3, 10, 50, torch.float32, 13, True)
+    _, (tol, (_, tol_x, tol_b)) = class_log_prob(
+        w, X, y, b, None, torch.ones(3, device='cuda'))
+    lp, (gw, gx, gb) = run(w, X, y, b, torch.ones(3, device='cuda'))
+    h = 2.0 ** -6
+    for d in range(10):
+        e = torch.zeros(10, device='cuda')
+        e[d] = h
+        up = zs.linear_categorical_log_prob(w, X + e, y, bias=b)
+        dn = zs.linear_categorical_log_prob(w, X - e, y, bias=b)
+        m = 2 * w[:, d].abs().max().double() ** 3
+        # (X +- h is itself rounded: at most 2^-24 |X +- h| |w| off)
+        slack = 2 ** -23 * (X[:, d].abs() + h).double() * \
+            w[:, d].abs().max().double()
+        assert bool(((up.double() - dn.double()) / (2 * h) -
+                     gx[:, d].double()).abs().le(
+            (2 * tol + 2 * slack) / (2 * h) + h * h / 6 * m +
+            tol_x[:, d]).all())
+    for v in (0, 17, 49):
+        e = torch.zeros(50, device='cuda')
+        e[v] = h
+        up = zs.linear_categorical_log_prob(w, X, y, bias=b + e).double().sum()
+        dn = zs.linear_categorical_log_prob(w, X, y, bias=b - e).double().sum()
+        t = float(tol.sum()) + 3 * 2 ** -23 * (float(b[v].abs()) + h)
+        assert abs(float((up - dn) / (2 * h) - gb[v].double())) <= \
+            2 * t / (2 * h) + 3 * h * h / 6 + float(tol_b[v])
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_same_bits_again_and_on_another_stream(dtype):
+    w, X, y, b, g = problem(200, 128, 3000, dtype, 14, True)
+    ref = run(w, X, y, b, g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(w, X, y, b, g)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, c in zip((got[0],) + got[1], (ref[0],) + ref[1]):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
+def test_captured_and_replayed(dtype):
+    """Forward and gradient in one graph, replayed over new inputs with other
+    work between."""
+    w, X, y, b, g = problem(150, 64, 2000, dtype, 15, True, IGNORE)
+    w, X, b = (t.requires_grad_() for t in (w, X, b))
+
+    def step():
+        lp = zs.linear_categorical_log_prob(w, X, y, bias=b,
+                                            ignore_label=IGNORE)
+        return (lp.detach(),) + torch.autograd.grad(lp, (w, X, b), g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        w2, X2, y2, b2, g2 = problem(150, 64, 2000, dtype, 20 + seed, True,
+                                     IGNORE)
+        with torch.no_grad():
+            for dst, src in ((w, w2), (X, X2), (y, y2), (b, b2), (g, g2)):
+                dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, step()):
+            assert torch.equal(a, c)
+        torch.randn(1000, 1000, device='cuda').sum().item()

@@ -10,7 +10,8 @@ from .framework import (BayesianNet, MetaBayesianNet, StochasticTensor,
                         meta_bayesian_net)
 from .distributions import (linear_class_logits, linear_logits,
                             log_mixture)
-from ._ops import gathered_dot, clear_caches
+from ._ops import (gathered_dot, clear_caches, linear_categorical_log_prob,
+                   QuantizedRows, quantize_rows, quantized_linear)
 from .evaluation import AIS
 from .hmc import (HMC, HMCInfo, InvalidArgumentError,
                   NativePlanFallbackWarning, LikelihoodArithmeticWarning,
@@ -24,4 +25,6 @@ __version__ = '0.1.0'
 __all__ = ['SGMCMC', 'SGLD', 'PSGLD', 'SGHMC', 'SGNHT', 'AIS', 'evaluation', 'HMC', 'HMCInfo', 'InvalidArgumentError', 'NativePlanFallbackWarning', 'LikelihoodArithmeticWarning', 'placeholder', 'deferred', 'Session',
            'BayesianNet', 'MetaBayesianNet', 'StochasticTensor',
            'meta_bayesian_net', 'distributions', 'diagnostics', 'framework',
-           'merge_dicts', 'set_random_seed', 'linear_logits', 'linear_class_logits', 'log_mixture', 'gathered_dot', 'clear_caches']
+           'merge_dicts', 'set_random_seed', 'linear_logits', 'linear_class_logits', 'log_mixture', 'gathered_dot', 'clear_caches',
+           'linear_categorical_log_prob', 'QuantizedRows', 'quantize_rows',
+           'quantized_linear']

@@ -109,6 +109,9 @@ BCAST_FULL = 0
 BCAST_ROW = 1
 BCAST_SCALAR = 2
 
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+
 _p = c_void_p  # every device pointer / stream travels as void*
 
 # name -> (restype, argtypes); mirrors include/zshmc.h one to one
@@ -264,6 +267,22 @@ PROTOTYPES = {
         _p, _p, c_int64, c_int64, c_uint64, c_uint32, _p]),
     'zshmc_categorical_sample': (c_int, [
         _p, _p, c_int64, c_int64, c_int64, c_uint64, c_uint32, _p]),
+    'zshmc_class_log_prob_workspace': (c_int, [
+        _p, _p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
+        c_int, _p]),
+    'zshmc_class_log_prob': (c_int, [
+        _p, _p, _p, _p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
+        c_int, c_int64, _p, _p, _p, c_int64, _p]),
+    'zshmc_class_log_prob_grad': (c_int, [
+        _p, _p, _p, _p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
+        c_int, c_int64, _p, _p, _p, _p, _p, _p, c_int64, _p]),
+    'zshmc_quantize_rows': (c_int, [
+        _p, c_int64, c_int64, c_int64, c_int, _p, c_int64, _p, _p]),
+    'zshmc_dequantize_rows': (c_int, [
+        _p, c_int64, _p, c_int64, c_int64, _p, c_int64, c_int, _p]),
+    'zshmc_int8_linear': (c_int, [
+        _p, c_int64, _p, _p, c_int64, _p, _p, c_int64, c_int64, c_int64, _p,
+        c_int64, c_int, _p]),
 }
 
 

@@ -990,3 +990,319 @@ class MixtureMultinomialLogLik(_Function):
         k = ctx.t_shape[-1]
         g = gt[:, :k] * gout.reshape(-1, 1)
         return g.reshape(ctx.t_shape), None, None
+
+
+# ----------------------------------------------------------------------------
+# linear output layers over many classes (csrc/class_logits.hip) and 8-bit rows
+# (csrc/int8_linear.hip)
+# ----------------------------------------------------------------------------
+_ROW_DTYPES = {torch.float32: _capi.DTYPE_F32, torch.bfloat16: _capi.DTYPE_BF16}
+
+
+def row_dtype(dtype, what):
+    """The C-ABI's code of an operand type."""
+    if dtype not in _ROW_DTYPES:
+        raise TypeError("{} must be float32 or bfloat16, got {}".format(
+            what, dtype))
+    return _ROW_DTYPES[dtype]
+
+
+def _rows_2d(t):
+    """t [..., K] as a matrix whose rows are contiguous (a view where t's
+    strides allow one), and its row stride in elements."""
+    t2 = t.detach().reshape(-1, t.shape[-1])
+    if t2.shape[0] > 1:
+        if t2.stride(1) != 1 and t2.shape[1] > 1 or t2.stride(0) < t2.shape[1]:
+            t2 = t2.contiguous()
+        return t2, max(int(t2.stride(0)), int(t2.shape[1]))
+    if t2.shape[1] > 1 and t2.stride(1) != 1:
+        t2 = t2.contiguous()
+    return t2, int(t2.shape[1])
+
+
+class ClassLogProb(_Function):
+    """log Categorical(labels | w X^T + bias) per row of X [N, D] and its
+    gradients for w [V, D], X and bias [V]; the [N, V] logits are never kept
+    (zshmc_class_log_prob; reference univariate.py:496-548)."""
+
+    @staticmethod
+    def forward(ctx, w, X, labels, bias, ignore_label):
+        w2, ldw = _rows_2d(w)
+        x2, ldx = _rows_2d(X)
+        b = None if bias is None else bias.detach().to(_F32).contiguous()
+        y = labels.detach().to(torch.int64).contiguous()
+        N, D, V = x2.shape[0], x2.shape[1], w2.shape[0]
+        ctx.dims = (N, D, V, ldx, ldw, row_dtype(w.dtype, 'w'),
+                    0 if ignore_label is None else 1, ignore_label or 0)
+        ctx.shapes = (tuple(w.shape), tuple(X.shape),
+                      None if bias is None else bias.dtype)
+        out = torch.empty(N, dtype=_F32, device=X.device)
+        need = any(ctx.needs_input_grad)
+        stats = torch.empty(N, 2, dtype=_F32, device=X.device) if need \
+            else None
+        with torch.cuda.device(X.device):
+            ws = ClassLogProb._workspace(x2, w2, ctx.dims, 0)
+            _capi.call('zshmc_class_log_prob', x2.data_ptr(), w2.data_ptr(),
+                       _capi.ptr(b), y.data_ptr(), *(ctx.dims + (
+                           out.data_ptr(), _capi.ptr(stats), ws.data_ptr(),
+                           ws.numel(), _capi.current_stream())))
+        if need:
+            ctx.save_for_backward(w, X, y, b, stats)
+        return out
+
+    @staticmethod
+    def _workspace(x2, w2, dims, gradient):
+        import ctypes
+        N, D, V, ldx, ldw, dtype, has_ignore, _ = dims
+        n = ctypes.c_int64(0)
+        _capi.call('zshmc_class_log_prob_workspace', x2.data_ptr(),
+                   w2.data_ptr(), N, D, V, ldx, ldw, dtype, gradient,
+                   has_ignore, ctypes.addressof(n))
+        return torch.empty(max(int(n.value), 16), dtype=torch.uint8,
+                           device=x2.device)
+
+    @staticmethod
+    def backward(ctx, gout):
+        w, X, y, b, stats = ctx.saved_tensors
+        (w2, _), (x2, _) = _rows_2d(w), _rows_2d(X)
+        w_shape, x_shape, b_dtype = ctx.shapes
+        need_w, need_x, _, need_b = ctx.needs_input_grad[:4]
+        g = gout.to(_F32).contiguous()
+        gw = torch.empty(w_shape, dtype=w.dtype, device=w.device) \
+            if need_w else None
+        gx = torch.empty(x_shape, dtype=X.dtype, device=X.device) \
+            if need_x else None
+        gb = torch.empty(w_shape[0], dtype=_F32, device=w.device) \
+            if need_b else None
+        with torch.cuda.device(X.device):
+            ws = ClassLogProb._workspace(x2, w2, ctx.dims, 1)
+            _capi.call('zshmc_class_log_prob_grad', x2.data_ptr(),
+                       w2.data_ptr(), _capi.ptr(b), y.data_ptr(),
+                       *(ctx.dims + (
+                           stats.data_ptr(), g.data_ptr(), _capi.ptr(gx),
+                           _capi.ptr(gw), _capi.ptr(gb), ws.data_ptr(),
+                           ws.numel(), _capi.current_stream())))
+        return (gw, gx, None, gb.to(b_dtype) if need_b else None, None)
+
+
+def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
+    """Log-probabilities of `labels` [...] under a Categorical whose logits
+    are a linear map, `X @ w^T + bias`, for many classes: X [..., D] and
+    w [V, D] float32 or bfloat16 (the same), integer labels of X's leading
+    shape, bias [V].  Returns float32 [...].  Differentiable in w, X and bias.
+
+    What `Categorical(logits=X @ w.T + bias).log_prob(labels)` computes, without the
+    [..., V] logits: the classes are taken in pieces in both directions.
+    float32 operands are multiplied with float32-level accuracy, bfloat16 ones as they
+    are; sums and the softmax statistics are float32 either way.
+
+    A row labelled `ignore_label` has the log-probability 0 and no part in any
+    gradient, whatever X holds there.  Any other label outside [0, V) gives
+    NaN (no host synchronisation to look for one).  Empty X is allowed."""
+    w, X, labels, bias = [
+        _symbolic.force(t.tensor if hasattr(t, 'tensor') else t)
+        for t in (w, X, labels, bias)]
+    for name, t in (('w', w), ('X', X), ('labels', labels)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("linear_categorical_log_prob: {} must be a tensor"
+                            .format(name))
+    row_dtype(w.dtype, 'linear_categorical_log_prob: w')
+    if X.dtype != w.dtype:
+        raise TypeError("linear_categorical_log_prob: X and w must have the "
+                        "same dtype, got {} and {}".format(X.dtype, w.dtype))
+    if labels.dtype not in (torch.int32, torch.int64):
+        raise TypeError("linear_categorical_log_prob: labels must be int32 or "
+                        "int64, got {}".format(labels.dtype))
+    if w.dim() != 2 or X.dim() < 1 or w.shape[0] == 0 or \
+            w.shape[1] == 0 or X.shape[-1] != w.shape[1]:
+        raise ValueError("linear_categorical_log_prob: w [V, D] and X [..., D]"
+                         " expected, got {} and {}".format(tuple(w.shape),
+                                                           tuple(X.shape)))
+    if tuple(labels.shape) != tuple(X.shape[:-1]):
+        raise ValueError("linear_categorical_log_prob: labels {} for X {}"
+                         .format(tuple(labels.shape), tuple(X.shape)))
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or \
+                bias.dtype not in (torch.float32, w.dtype):
+            raise TypeError("linear_categorical_log_prob: bias must be a "
+                            "float32 tensor or of w's dtype")
+        if tuple(bias.shape) != (w.shape[0],):
+            raise ValueError("linear_categorical_log_prob: bias {} for {} "
+                             "classes".format(tuple(bias.shape), w.shape[0]))
+    require_device(w, X, labels, bias)
+    if any(t is not None and t.device != X.device for t in (w, labels, bias)):
+        raise ValueError("linear_categorical_log_prob: all tensors must be on "
+                         "one device")
+    if ignore_label is not None:
+        ignore_label = int(ignore_label)
+    out = ClassLogProb.apply(w, X.reshape(-1, X.shape[-1]),
+                             labels.reshape(-1), bias, ignore_label)
+    return out.reshape(labels.shape)
+
+
+class QuantizedRows(object):
+    """A matrix [..., K] as 8-bit integers with one float32 scale per row,
+    x ~ values * scale: what `quantize_rows` returns and `quantized_linear`
+    multiplies.  `values` int8 [..., K], `scale` float32 [...].  Values in
+    rows of whole, aligned 16 bytes are used where they lie (a later write to
+    them is seen); others are copied into such rows here, once."""
+
+    def __init__(self, values, scale):
+        if not isinstance(values, torch.Tensor) or \
+                not isinstance(scale, torch.Tensor) or \
+                values.dtype != torch.int8 or scale.dtype != _F32:
+            raise TypeError("QuantizedRows: int8 values and float32 scale "
+                            "tensors expected")
+        if values.dim() < 1 or values.shape[-1] == 0 or \
+                tuple(scale.shape) != tuple(values.shape[:-1]):
+            raise ValueError("QuantizedRows: values [..., K] and scale [...] "
+                             "expected, got {} and {}".format(
+                                 tuple(values.shape), tuple(scale.shape)))
+        require_device(values, scale)
+        if values.device != scale.device:
+            raise ValueError("QuantizedRows: values and scale must be on one "
+                             "device")
+        self._shape = values.shape
+        K = int(values.shape[-1])
+        rows = values.reshape(-1, K)
+        if not self._usable(rows):
+            rows = self._padded(rows)
+        self._rows, self.scale = rows, scale
+        self._flat_scale = scale.reshape(-1).contiguous()
+        # zeros behind the last column, as the left operand needs them
+        self._zero_tail = K % 16 == 0
+
+    @staticmethod
+    def _usable(rows):
+        """Rows of whole 16 bytes, readable to their end."""
+        n, K = rows.shape
+        if n == 0:
+            return False
+        pitch = rows.stride(0) if n > 1 else (K + 15) // 16 * 16
+        end = rows.storage_offset() + (n - 1) * pitch + (K + 15) // 16 * 16
+        return ((K == 1 or rows.stride(1) == 1) and pitch % 16 == 0 and
+                pitch >= (K + 15) // 16 * 16 and
+                rows.data_ptr() % 16 == 0 and
+                end <= rows.untyped_storage().nbytes())
+
+    @staticmethod
+    def _empty(n, K, device):
+        """int8 [n, K] at a pitch of whole 128 bytes, a view of its storage."""
+        return torch.empty(n, (K + 127) // 128 * 128, dtype=torch.int8,
+                           device=device)[:, :K]
+
+    @classmethod
+    def _padded(cls, rows):
+        n, K = rows.shape
+        out = torch.zeros(n, (K + 127) // 128 * 128, dtype=torch.int8,
+                          device=rows.device)[:, :K]
+        out.copy_(rows)
+        return out
+
+    @property
+    def values(self):
+        return self._rows.reshape(self._shape) if len(self._shape) != 2 \
+            else self._rows
+
+    @property
+    def shape(self):
+        return self._shape
+
+    @property
+    def device(self):
+        return self._rows.device
+
+    @property
+    def pitch(self):
+        return int(self._rows.stride(0)) if self._rows.shape[0] > 1 else \
+            (int(self._shape[-1]) + 15) // 16 * 16
+
+    def dequantize(self, dtype=torch.float32):
+        """values * scale as a dense tensor."""
+        code = row_dtype(dtype, 'dequantize: dtype')
+        out = torch.empty(self._shape, dtype=dtype, device=self.device)
+        n, K = self._rows.shape
+        if n:
+            with torch.cuda.device(self.device):
+                _capi.call('zshmc_dequantize_rows', self._rows.data_ptr(),
+                           self.pitch, self._flat_scale.data_ptr(), n, K,
+                           out.data_ptr(), K, code, _capi.current_stream())
+        return out
+
+
+def quantize_rows(x):
+    """x [..., K] (float32 or bfloat16) rounded to 8-bit integers with one
+    scale per row, `scale = max|x| / 127` over the row and `values =
+    rint(x / scale)` (to even): a `QuantizedRows`.  A row of zeros has the
+    scale 1; a row with an infinity or a NaN has the scale NaN.  No gradient."""
+    x = _symbolic.force(x.tensor if hasattr(x, 'tensor') else x)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("quantize_rows: a tensor expected")
+    code = row_dtype(x.dtype, 'quantize_rows: x')
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("quantize_rows: x [..., K] with K > 0 expected, got "
+                         "{}".format(tuple(x.shape)))
+    require_device(x)
+    x2, ldx = _rows_2d(x)
+    n, K = x2.shape
+    rows = QuantizedRows._empty(n, K, x.device)
+    scale = torch.empty(n, dtype=_F32, device=x.device)
+    if n:
+        with torch.cuda.device(x.device):
+            _capi.call('zshmc_quantize_rows', x2.data_ptr(), n, K, ldx, code,
+                       rows.data_ptr(), (K + 127) // 128 * 128,
+                       scale.data_ptr(), _capi.current_stream())
+    q = QuantizedRows.__new__(QuantizedRows)
+    q._shape, q._rows, q._zero_tail = x.shape, rows, True
+    q._flat_scale, q.scale = scale, scale.reshape(x.shape[:-1])
+    return q
+
+
+def quantized_linear(w, X, bias=None, dtype=None):
+    """`X @ w^T + bias` in 8-bit integers: w a `QuantizedRows` [V, K] (one
+    scale per output channel), X [..., K] a float32 / bfloat16 tensor -- rounded
+    to 8 bits per row here -- or a `QuantizedRows`.  The integer sum is exact;
+    out[..., v] = (scale_x scale_w[v]) * sum + bias[v] in float32, rounded once to
+    `dtype` (X's own, float32 for a QuantizedRows).  K <= 131072.  No gradient."""
+    if not isinstance(w, QuantizedRows) or len(w.shape) != 2:
+        raise TypeError("quantized_linear: w must be QuantizedRows [V, K]")
+    X = _symbolic.force(X.tensor if hasattr(X, 'tensor') else X)
+    if not isinstance(X, (torch.Tensor, QuantizedRows)):
+        raise TypeError("quantized_linear: X must be a tensor or QuantizedRows")
+    if dtype is None:
+        dtype = X.dtype if isinstance(X, torch.Tensor) else _F32
+    code = row_dtype(dtype, 'quantized_linear: dtype')
+    V, K = w.shape
+    if len(X.shape) < 1 or X.shape[-1] != K or V == 0:
+        raise ValueError("quantized_linear: w [V, K] and X [..., K] expected, "
+                         "got {} and {}".format(tuple(w.shape),
+                                                tuple(X.shape)))
+    if K > 131072:
+        raise ValueError("quantized_linear: at most 131072 columns (the sum "
+                         "is an int32), got {}".format(K))
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or not \
+                bias.dtype.is_floating_point or tuple(bias.shape) != (V,):
+            raise ValueError("quantized_linear: bias must be a float tensor "
+                             "[{}]".format(V))
+        require_device(bias)
+        bias = bias.detach().to(_F32).contiguous()
+    if isinstance(X, torch.Tensor):
+        require_device(X)
+    if any(t is not None and t.device != w.device for t in (X, bias)):
+        raise ValueError("quantized_linear: all tensors must be on one device")
+    x = quantize_rows(X) if isinstance(X, torch.Tensor) else X
+    rows, pitch = x._rows, x.pitch
+    if not x._zero_tail:
+        rows = QuantizedRows._padded(rows)
+        pitch = int(rows.stride(0))
+    out = torch.empty(tuple(x.shape[:-1]) + (V,), dtype=dtype,
+                      device=w.device)
+    if rows.shape[0]:
+        with torch.cuda.device(w.device):
+            _capi.call('zshmc_int8_linear', rows.data_ptr(), pitch,
+                       x._flat_scale.data_ptr(), w._rows.data_ptr(), w.pitch,
+                       w._flat_scale.data_ptr(), _capi.ptr(bias),
+                       rows.shape[0], K, V, out.data_ptr(), V, code,
+                       _capi.current_stream())
+    return out

@@ -1,0 +1,328 @@
+// The tile loop shared by the linear-Categorical kernels (csrc/class_logits.hip)
+// and the 8-bit products (csrc/int8_linear.hip): one workgroup of four waves
+// accumulates a BM x BN block of C[m, n] = sum_k A[m, k] B[n, k] on the matrix
+// cores, with operands of 128 bytes of k per step.
+//
+// Both operands travel global -> LDS by DMA (buffer_load ... lds, 16 bytes a
+// lane).  The buffer descriptor carries the bounds: rows past the operand's end
+// and, through the lane's own offset, columns past its k range arrive as zeros,
+// so odd sizes need no other code.  An operand is stored in one of two ways:
+//   k-contiguous ("kc"): row m holds its k's side by side.  LDS row m is 128
+//     bytes; its eight 16-byte chunks are rotated by XOR with (m >> 1) & 7, so
+//     that the 16 lanes that a ds_read_b128 serves at a time (rows {0-3, 12-15,
+//     20-27} / {4-11, 16-19, 28-31} of a 32-row block) touch all 64 banks once.
+//   k-major ("km", 2-byte elements): row k holds the m's side by side.  The LDS
+//     row k is BM (BN) elements and the fragment is taken by the transposing
+//     read ds_read_b64_tr_b16, 4 k's x 16 m's per group of 16 lanes; chunks are
+//     XORed with 4 (k & 3) so that the four k rows of a read sit in different
+//     quarters of the banks.  The gradient products contract over rows this
+//     way and no operand is ever transposed in memory.
+// A step's four MFMA k-slices (kk) are software-pipelined over two register
+// sets; the one barrier of a step sits in front of its LAST slice, whose
+// operands are in registers by then: the DMA of the step after next and the
+// first reads of the next step go out under the last slice's MFMAs.
+//
+// `terms`: float32 operands come as three bfloat16 planes (x = hi + mid + lo,
+// exact) and a product is the six plane pairs whose weight is above 2^-24:
+// the loop runs over the pairs, smallest first, into the same float32
+// accumulators.  One pair otherwise.
+#pragma once
+#include "common.h"
+
+namespace zshmc {
+
+typedef unsigned int tu4 __attribute__((ext_vector_type(4)));
+typedef unsigned int tu2 __attribute__((ext_vector_type(2)));
+typedef int ti4 __attribute__((ext_vector_type(4)));
+typedef short ts4 __attribute__((ext_vector_type(4)));
+typedef float tf4 __attribute__((ext_vector_type(4)));
+typedef float tf16 __attribute__((ext_vector_type(16)));
+typedef int ti16 __attribute__((ext_vector_type(16)));
+typedef __bf16 tb8 __attribute__((ext_vector_type(8)));
+#define ZS_TLDS __attribute__((address_space(3)))
+
+// One operand as it lies in memory: rows x row_bytes, `pitch` bytes apart
+// (both multiples of 16, base too), `plane` bytes from one plane to the next.
+struct TileOperand {
+  const unsigned char* base;
+  int64_t pitch, plane;
+  int64_t rows, row_bytes;
+};
+
+// plane pairs, two bits each, smallest product first; bf16 / int8 use pair 0
+// of one term (hi x hi)
+constexpr int kTerms3 = 6;
+constexpr uint32_t kTermsA3 = 1u | 2u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+constexpr uint32_t kTermsB3 = 1u | 0u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+
+struct MmaBf16 {
+  typedef tf16 Acc;
+  static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(tb8, a), __builtin_bit_cast(tb8, b), c, 0, 0, 0);
+  }
+};
+struct MmaI8 {
+  typedef ti16 Acc;
+  static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(
+        __builtin_bit_cast(ti4, a), __builtin_bit_cast(ti4, b), c, 0, 0, 0);
+  }
+};
+
+// 16 bytes of a row that may start anywhere (global memory takes such accesses
+// at its elements' alignment)
+typedef unsigned int tu4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int tu2_any __attribute__((ext_vector_type(2), aligned(2)));
+
+// 16 bytes a lane, global -> LDS at lds + 16 * lane
+__device__ __forceinline__ void tile_dma16(const tu4& srd, uint32_t voff, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(voff), "s"(srd), "s"(lds)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tile_wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// WGM x WGN waves (four), each WM x WN blocks of 32 x 32
+template <typename MMA_, int WGM_, int WGN_, int WM_, int WN_, bool A_KM_, bool B_KM_,
+          int NBUF_>
+struct TileCfg {
+  typedef MMA_ MMA;
+  static constexpr int WGM = WGM_, WGN = WGN_, WM = WM_, WN = WN_, NBUF = NBUF_;
+  static constexpr bool A_KM = A_KM_, B_KM = B_KM_;
+  static constexpr int BM = WGM * WM * 32, BN = WGN * WN * 32;
+  static constexpr int kStage = (BM + BN) * 128;
+  static constexpr int kLds = NBUF * kStage;
+  static_assert(WGM * WGN == 4, "four waves");
+  static_assert(!A_KM || BM == 128 || BM == 256, "whole rows per DMA piece");
+  static_assert(!B_KM || BN == 128 || BN == 256, "whole rows per DMA piece");
+};
+
+// One operand's side of a step: its DMA lane offsets and its LDS fragments.
+// ROWS: BM or BN; OFF: its place in a stage; NB: 32-blocks of the wave.
+template <bool KM, int ROWS, int OFF, int NB>
+struct TileSide {
+  static constexpr int kPieces = ROWS / 8 / 4;     // 1 KB pieces per wave
+  uint32_t voff[kPieces];
+  uint32_t chunk16;          // kc: the lane's chunk offset within 128 bytes
+  uint32_t frag[KM ? NB : 4];
+  int64_t step_bytes;
+  const unsigned char* base;
+  int64_t pitch, plane, rows_left, bytes_left;
+
+  // row0: first m (n) of the tile; k0: first step
+  __device__ __forceinline__ void init(const TileOperand& o, int64_t row0, int k0,
+                                       int lane, int wave, int blk0) {
+    pitch = o.pitch;
+    plane = o.plane;
+    if constexpr (!KM) {
+      const int sub = lane >> 3;
+      const int f = (4 * (wave & 1) + (sub >> 1)) & 7;
+      chunk16 = (uint32_t)(((lane & 7) ^ f) * 16);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+        voff[j] = (uint32_t)((8 * (wave + 4 * j) + sub) * pitch) + chunk16;
+      base = o.base + row0 * pitch + (int64_t)k0 * 128;
+      rows_left = o.rows - row0 < ROWS ? o.rows - row0 : ROWS;
+      bytes_left = o.row_bytes - (int64_t)k0 * 128;
+      step_bytes = 128;
+      const uint32_t r = OFF + (blk0 * 32 + (lane & 31)) * 128;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        frag[kk] = r + (uint32_t)(((2 * kk + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16);
+    } else {
+      constexpr int CR = ROWS / 8;                 // chunks per LDS row
+      constexpr int RP = 64 / CR;                  // rows per piece
+      const int sub = lane / CR;
+      const int row3 = (RP * wave + sub) & 3;
+      const uint32_t c = (uint32_t)((lane % CR) ^ (4 * row3));
+      chunk16 = 0;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+        voff[j] = (uint32_t)((RP * (wave + 4 * j) + sub) * pitch) + c * 16;
+      base = o.base + (int64_t)k0 * 64 * pitch + row0 * 2;
+      rows_left = o.rows - (int64_t)k0 * 64;
+      bytes_left = o.row_bytes - row0 * 2;
+      step_bytes = 64 * pitch;
+      const int k3 = (lane & 15) >> 2;
+      const uint32_t kr = OFF + (uint32_t)(((lane >> 5) * 8 + k3) * (ROWS * 2)) + (lane & 1) * 8;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int ch = (blk0 + b) * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+        frag[b] = kr + (uint32_t)((ch ^ (4 * k3)) * 16);
+      }
+    }
+  }
+  // the DMA of step `ks` (counted from init's k0) of plane `pl`
+  __device__ __forceinline__ void issue(int pl, int ks, uint32_t lds, int wave) const {
+    const unsigned char* p = base + pl * plane + ks * step_bytes;
+    int64_t n;
+    bool cut = false;
+    uint32_t left = 128;
+    if constexpr (!KM) {
+      const int64_t l = bytes_left - (int64_t)ks * 128;
+      n = (rows_left - 1) * pitch + l;
+      cut = l < 128;
+      left = (uint32_t)l;
+    } else {
+      const int64_t r = rows_left - (int64_t)ks * 64;
+      n = ((r < 64 ? r : 64) - 1) * pitch + bytes_left;
+    }
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    tu4 srd;
+    srd[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    srd[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+    srd[2] = __builtin_amdgcn_readfirstlane((uint32_t)n);
+    srd[3] = 0x00020000u;
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      uint32_t v = voff[j];
+      if (cut) v = chunk16 >= left ? 0xffffff00u : v;
+      tile_dma16(srd, v, lds + (uint32_t)(OFF + (wave + 4 * j) * 1024));
+    }
+  }
+  __device__ __forceinline__ void read(tu4 (&f)[NB], uint32_t stage, int kk) const {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if constexpr (!KM) {
+        f[b] = *reinterpret_cast<const ZS_TLDS tu4*>(
+            (uintptr_t)(stage + frag[kk] + (uint32_t)(b * 4096)));
+      } else {
+        const uint32_t at = stage + frag[b] + (uint32_t)(kk * 16 * ROWS * 2);
+        const tu2 lo = __builtin_bit_cast(
+            tu2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                     reinterpret_cast<ZS_TLDS ts4*>((uintptr_t)at)));
+        const tu2 hi = __builtin_bit_cast(
+            tu2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                     reinterpret_cast<ZS_TLDS ts4*>((uintptr_t)(at + 4 * ROWS * 2))));
+        f[b] = tu4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    }
+  }
+};
+
+// acc = sum over `terms` plane pairs and `steps` k-steps from k0 on.  Leaves
+// with every DMA landed and every wave past its last LDS read.
+template <typename C>
+__device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperand& B,
+                                          int64_t m0, int64_t n0, int k0, int steps, int terms,
+                                          uint32_t lds, int lane, int wave,
+                                          typename C::MMA::Acc (&acc)[C::WM][C::WN]) {
+  typedef TileSide<C::A_KM, C::BM, 0, C::WM> SideA;
+  typedef TileSide<C::B_KM, C::BN, C::BM * 128, C::WN> SideB;
+  constexpr int PW = SideA::kPieces + SideB::kPieces;
+  constexpr int NBUF = C::NBUF;
+  SideA sa;
+  SideB sb;
+  sa.init(A, m0, k0, lane, wave, (wave / C::WGN) * C::WM);
+  sb.init(B, n0, k0, lane, wave, (wave % C::WGN) * C::WN);
+#pragma unroll
+  for (int i = 0; i < C::WM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::WN; ++j) acc[i][j] = typename C::MMA::Acc{};
+
+  const int total = terms * steps;
+  const uint32_t ta = terms > 1 ? kTermsA3 : 0u, tb = terms > 1 ? kTermsB3 : 0u;
+  int it = 0, ik = 0, ibuf = 0;          // the next step to issue: term, k-step, buffer
+  auto issue = [&]() {
+    const uint32_t dst = lds + (uint32_t)(ibuf * C::kStage);
+    sa.issue((ta >> (2 * it)) & 3, ik, dst, wave);
+    sb.issue((tb >> (2 * it)) & 3, ik, dst, wave);
+    if (++ik == steps) ik = 0, ++it;
+    if (++ibuf == NBUF) ibuf = 0;
+  };
+  tu4 fa[2][C::WM], fb[2][C::WN];
+  auto multiply = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < C::WM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::WN; ++j)
+        acc[i][j] = C::MMA::mma(fa[s][i], fb[s][j], acc[i][j]);
+  };
+  const int first = total < NBUF ? total : NBUF;
+  for (int t = 0; t < first; ++t) issue();
+  if (first == NBUF)
+    tile_wait_barrier<(NBUF - 1) * PW>();
+  else
+    tile_wait_barrier<0>();
+  uint32_t cur = lds;
+  sa.read(fa[0], cur, 0);
+  sb.read(fb[0], cur, 0);
+  int buf = 0;
+  for (int t = 0; t < total; ++t) {
+#pragma unroll
+    for (int kk = 0; kk < 3; ++kk) {
+      sa.read(fa[(kk + 1) & 1], cur, kk + 1);
+      sb.read(fb[(kk + 1) & 1], cur, kk + 1);
+      multiply(kk & 1);
+    }
+    if (t + 1 < total) {
+      // step t + 1 has landed (those behind it may be in flight), and every
+      // wave has its last slice of step t in registers: its buffer is free
+      if (t + NBUF <= total)
+        tile_wait_barrier<(NBUF - 2) * PW>();
+      else
+        tile_wait_barrier<0>();
+      if (t + NBUF < total) issue();
+      if (++buf == NBUF) buf = 0;
+      cur = lds + (uint32_t)(buf * C::kStage);
+      sa.read(fa[0], cur, 0);
+      sb.read(fb[0], cur, 0);
+    }
+    multiply(1);
+  }
+  tile_wait_barrier<0>();
+  // for acc_get: every MFMA is in front of these statements, and its 16 passes
+  // and the read's wait states behind the last
+#pragma unroll
+  for (int i = 0; i < C::WM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::WN; ++j) asm volatile("" : "+a"(acc[i][j]));
+  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+}
+
+// Workgroup -> tile.  Workgroups go round-robin over the eight XCDs, each with
+// an L2 of its own: every XCD takes a contiguous share of the tiles, ordered
+// in bands of eight tile rows, so that the ~32 tiles an XCD runs at a time
+// share eight row blocks and four column blocks of the operands.
+__device__ __forceinline__ void tile_of_block(uint32_t bid, uint32_t n_wg, uint32_t tiles_m,
+                                              uint32_t tiles_n, int& tm, int& tn) {
+  const uint32_t x = bid & 7u, idx = bid >> 3;
+  const uint32_t per = n_wg >> 3, rem = n_wg & 7u;
+  const uint32_t id = x * per + (x < rem ? x : rem) + idx;
+  const uint32_t band = id / (8u * tiles_n);
+  const uint32_t in = id - band * 8u * tiles_n;
+  const uint32_t rows = tiles_m - band * 8u < 8u ? tiles_m - band * 8u : 8u;
+  const uint32_t c = in / rows;
+  tm = __builtin_amdgcn_readfirstlane((int)(band * 8u + (in - c * rows)));
+  tn = __builtin_amdgcn_readfirstlane((int)c);
+}
+
+// row of a 32 x 32 accumulator block held in register r of lane half h
+__device__ __forceinline__ constexpr int acc_row(int r, int h) {
+  return (r & 3) + 8 * (r >> 2) + 4 * h;
+}
+
+// One accumulator element for the vector unit.  The accumulators of the large
+// tiles fill the AGPRs; read through the compiler, all of them move to VGPRs at
+// the loop's end, which spills.  This read names the AGPR in place.  tile_loop
+// ends with the wait states that such a read needs behind the last MFMA.
+__device__ __forceinline__ float acc_get(const tf16& v, int r) {
+  float x;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(v[r]));
+  return x;
+}
+__device__ __forceinline__ int acc_get(const ti16& v, int r) {
+  int x;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(v[r]));
+  return x;
+}
+
+}  // namespace zshmc

@@ -19,14 +19,26 @@
 //     way and no operand is ever transposed in memory.
 // A step's four MFMA k-slices (kk) are software-pipelined over two register
 // sets; the one barrier of a step sits in front of its LAST slice, whose
-// operands are in registers by then: the DMA of the step after next and the
-// first reads of the next step go out under the last slice's MFMAs.
+// operands are in registers by then.  Every slice is written in issue order: the
+// next slice's LDS reads in front of its first MFMAs, and the DMA of the step
+// NBUF ahead -- into the buffer that the barrier has just freed -- one piece at a
+// time between the MFMAs of the three slices behind the barrier (issued in one
+// burst, four waves' 64 pieces hold the memory pipe for ~1000 clocks and every
+// wave's in-order issue behind it).  Steps past the last are issued with an empty
+// descriptor (zeros, no memory traffic), so that the waits count the same
+// everywhere.  32768 x 4096 x 4096 bf16, 256 x 256 tiles: burst 1090 TFLOP/s, even
+// over all four slices 1130, over three with the MFMA waves' priority raised
+// 1385; eight waves of 128 x 64 each 1345, 64-byte steps in four buffers 1280,
+// two workgroups of 128 x 128 a CU 1105.
 //
 // `terms`: float32 operands come as three bfloat16 planes (x = hi + mid + lo,
 // exact) and a product is the six plane pairs whose weight is above 2^-24:
 // the loop runs over the pairs, smallest first, into the same float32
 // accumulators.  One pair otherwise.
 #pragma once
+#include <type_traits>
+#include <utility>
+
 #include "common.h"
 
 namespace zshmc {
@@ -89,6 +101,15 @@ template <int N>
 __device__ __forceinline__ void tile_wait_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+template <typename F, int... I>
+__device__ __forceinline__ void tile_for_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+// f(0), ..., f(N - 1) with the index a constant
+template <int N, typename F>
+__device__ __forceinline__ void tile_for(F&& f) {
+  tile_for_impl(f, std::make_integer_sequence<int, N>{});
+}
 
 // WGM x WGN waves (four), each WM x WN blocks of 32 x 32
 template <typename MMA_, int WGM_, int WGN_, int WM_, int WN_, bool A_KM_, bool B_KM_,
@@ -116,6 +137,9 @@ struct TileSide {
   int64_t step_bytes;
   const unsigned char* base;
   int64_t pitch, plane, rows_left, bytes_left;
+  tu4 srd;                   // the step that dma() fetches
+  bool cut;                  // ... ends inside its 128 bytes, at byte `left`
+  uint32_t left;
 
   // row0: first m (n) of the tile; k0: first step
   __device__ __forceinline__ void init(const TileOperand& o, int64_t row0, int k0,
@@ -160,12 +184,12 @@ struct TileSide {
       }
     }
   }
-  // the DMA of step `ks` (counted from init's k0) of plane `pl`
-  __device__ __forceinline__ void issue(int pl, int ks, uint32_t lds, int wave) const {
+  // step `ks` (counted from init's k0) of plane `pl` next; nothing if not `live`
+  __device__ __forceinline__ void aim(int pl, int ks, bool live) {
     const unsigned char* p = base + pl * plane + ks * step_bytes;
     int64_t n;
-    bool cut = false;
-    uint32_t left = 128;
+    cut = false;
+    left = 128;
     if constexpr (!KM) {
       const int64_t l = bytes_left - (int64_t)ks * 128;
       n = (rows_left - 1) * pitch + l;
@@ -176,34 +200,31 @@ struct TileSide {
       n = ((r < 64 ? r : 64) - 1) * pitch + bytes_left;
     }
     const uint64_t a = reinterpret_cast<uint64_t>(p);
-    tu4 srd;
     srd[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
     srd[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
-    srd[2] = __builtin_amdgcn_readfirstlane((uint32_t)n);
+    srd[2] = __builtin_amdgcn_readfirstlane(live ? (uint32_t)n : 0u);
     srd[3] = 0x00020000u;
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      uint32_t v = voff[j];
-      if (cut) v = chunk16 >= left ? 0xffffff00u : v;
-      tile_dma16(srd, v, lds + (uint32_t)(OFF + (wave + 4 * j) * 1024));
-    }
   }
-  __device__ __forceinline__ void read(tu4 (&f)[NB], uint32_t stage, int kk) const {
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      if constexpr (!KM) {
-        f[b] = *reinterpret_cast<const ZS_TLDS tu4*>(
-            (uintptr_t)(stage + frag[kk] + (uint32_t)(b * 4096)));
-      } else {
-        const uint32_t at = stage + frag[b] + (uint32_t)(kk * 16 * ROWS * 2);
-        const tu2 lo = __builtin_bit_cast(
-            tu2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                     reinterpret_cast<ZS_TLDS ts4*>((uintptr_t)at)));
-        const tu2 hi = __builtin_bit_cast(
-            tu2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                     reinterpret_cast<ZS_TLDS ts4*>((uintptr_t)(at + 4 * ROWS * 2))));
-        f[b] = tu4{lo[0], lo[1], hi[0], hi[1]};
-      }
+  // its j-th piece of this wave
+  __device__ __forceinline__ void dma(int j, uint32_t lds, int wave) const {
+    uint32_t v = voff[j];
+    if constexpr (!KM) v = cut && chunk16 >= left ? 0xffffff00u : v;
+    tile_dma16(srd, v, lds + (uint32_t)(OFF + (wave + 4 * j) * 1024));
+  }
+  // block b's fragment of slice kk
+  __device__ __forceinline__ void read(tu4& f, uint32_t stage, int kk, int b) const {
+    if constexpr (!KM) {
+      f = *reinterpret_cast<const ZS_TLDS tu4*>(
+          (uintptr_t)(stage + frag[kk] + (uint32_t)(b * 4096)));
+    } else {
+      const uint32_t at = stage + frag[b] + (uint32_t)(kk * 16 * ROWS * 2);
+      const tu2 lo = __builtin_bit_cast(
+          tu2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   reinterpret_cast<ZS_TLDS ts4*>((uintptr_t)at)));
+      const tu2 hi = __builtin_bit_cast(
+          tu2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   reinterpret_cast<ZS_TLDS ts4*>((uintptr_t)(at + 4 * ROWS * 2))));
+      f = tu4{lo[0], lo[1], hi[0], hi[1]};
     }
   }
 };
@@ -217,8 +238,8 @@ __device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperan
                                           typename C::MMA::Acc (&acc)[C::WM][C::WN]) {
   typedef TileSide<C::A_KM, C::BM, 0, C::WM> SideA;
   typedef TileSide<C::B_KM, C::BN, C::BM * 128, C::WN> SideB;
-  constexpr int PW = SideA::kPieces + SideB::kPieces;
-  constexpr int NBUF = C::NBUF;
+  constexpr int PA = SideA::kPieces, PW = PA + SideB::kPieces;
+  constexpr int NBUF = C::NBUF, M = C::WM * C::WN, R = C::WM + C::WN;
   SideA sa;
   SideB sb;
   sa.init(A, m0, k0, lane, wave, (wave / C::WGN) * C::WM);
@@ -230,54 +251,76 @@ __device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperan
 
   const int total = terms * steps;
   const uint32_t ta = terms > 1 ? kTermsA3 : 0u, tb = terms > 1 ? kTermsB3 : 0u;
-  int it = 0, ik = 0, ibuf = 0;          // the next step to issue: term, k-step, buffer
-  auto issue = [&]() {
-    const uint32_t dst = lds + (uint32_t)(ibuf * C::kStage);
-    sa.issue((ta >> (2 * it)) & 3, ik, dst, wave);
-    sb.issue((tb >> (2 * it)) & 3, ik, dst, wave);
+  // the next step to issue: its term, k-step and buffer
+  int issued = 0, it = 0, ik = 0, ibuf = 0;
+  uint32_t dst = lds;
+  auto aim = [&]() {
+    const bool live = issued < total;
+    sa.aim((ta >> (2 * it)) & 3, ik, live);
+    sb.aim((tb >> (2 * it)) & 3, ik, live);
+    dst = lds + (uint32_t)(ibuf * C::kStage);
+    ++issued;
     if (++ik == steps) ik = 0, ++it;
     if (++ibuf == NBUF) ibuf = 0;
   };
-  tu4 fa[2][C::WM], fb[2][C::WN];
-  auto multiply = [&](int s) {
-#pragma unroll
-    for (int i = 0; i < C::WM; ++i)
-#pragma unroll
-      for (int j = 0; j < C::WN; ++j)
-        acc[i][j] = C::MMA::mma(fa[s][i], fb[s][j], acc[i][j]);
+  auto dma = [&](int j) {
+    if (j < PA)
+      sa.dma(j, dst, wave);
+    else
+      sb.dma(j - PA, dst, wave);
   };
-  const int first = total < NBUF ? total : NBUF;
-  for (int t = 0; t < first; ++t) issue();
-  if (first == NBUF)
-    tile_wait_barrier<(NBUF - 1) * PW>();
-  else
-    tile_wait_barrier<0>();
+  tu4 fa[2][C::WM], fb[2][C::WN];
+  // The MFMAs of register set S, in between the reads of slice KK_ of `stage`
+  // into the other set and the pieces [D0, D1) of the step aimed at
+  auto slice = [&](auto S, uint32_t stage, auto KK, auto D0, auto D1) {
+    constexpr int s = decltype(S)::value, kk = decltype(KK)::value;
+    constexpr int d0 = decltype(D0)::value, nd = decltype(D1)::value - d0;
+    tile_for<M>([&](auto M_) {
+      constexpr int m = decltype(M_)::value;
+      tile_for<R>([&](auto Q) {
+        constexpr int q = decltype(Q)::value;
+        if constexpr (q * M / R == m) {
+          if constexpr (q < C::WN)
+            sb.read(fb[s ^ 1][q], stage, kk, q);
+          else
+            sa.read(fa[s ^ 1][q - C::WN], stage, kk, q - C::WN);
+        }
+      });
+      tile_for<nd>([&](auto Q) {
+        constexpr int q = decltype(Q)::value;
+        if constexpr (q * M / nd == m) dma(d0 + q);
+      });
+      constexpr int i = m / C::WN, j = m % C::WN;
+      if constexpr (m == 0) __builtin_amdgcn_s_setprio(1);
+      acc[i][j] = C::MMA::mma(fa[s][i], fb[s][j], acc[i][j]);
+      if constexpr (m == M - 1) __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+#define ZS_IC(x) std::integral_constant<int, (x)>{}
+  for (int t = 0; t < NBUF; ++t) {
+    aim();
+#pragma unroll
+    for (int j = 0; j < PW; ++j) dma(j);
+  }
+  tile_wait_barrier<(NBUF - 1) * PW>();
   uint32_t cur = lds;
-  sa.read(fa[0], cur, 0);
-  sb.read(fb[0], cur, 0);
+  tile_for<C::WN>([&](auto Q) { sb.read(fb[0][decltype(Q)::value], cur, 0, decltype(Q)::value); });
+  tile_for<C::WM>([&](auto Q) { sa.read(fa[0][decltype(Q)::value], cur, 0, decltype(Q)::value); });
   int buf = 0;
   for (int t = 0; t < total; ++t) {
-#pragma unroll
-    for (int kk = 0; kk < 3; ++kk) {
-      sa.read(fa[(kk + 1) & 1], cur, kk + 1);
-      sb.read(fb[(kk + 1) & 1], cur, kk + 1);
-      multiply(kk & 1);
-    }
-    if (t + 1 < total) {
-      // step t + 1 has landed (those behind it may be in flight), and every
-      // wave has its last slice of step t in registers: its buffer is free
-      if (t + NBUF <= total)
-        tile_wait_barrier<(NBUF - 2) * PW>();
-      else
-        tile_wait_barrier<0>();
-      if (t + NBUF < total) issue();
-      if (++buf == NBUF) buf = 0;
-      cur = lds + (uint32_t)(buf * C::kStage);
-      sa.read(fa[0], cur, 0);
-      sb.read(fb[0], cur, 0);
-    }
-    multiply(1);
+    slice(ZS_IC(0), cur, ZS_IC(1), ZS_IC(PW / 3), ZS_IC(PW * 2 / 3));
+    slice(ZS_IC(1), cur, ZS_IC(2), ZS_IC(PW * 2 / 3), ZS_IC(PW));
+    slice(ZS_IC(0), cur, ZS_IC(3), ZS_IC(0), ZS_IC(0));
+    // step t + 1 has landed (those behind it may be in flight), and every wave
+    // has its last slice of step t in registers: its buffer is free
+    tile_wait_barrier<(NBUF - 2) * PW>();
+    if (++buf == NBUF) buf = 0;
+    cur = lds + (uint32_t)(buf * C::kStage);
+    aim();
+    slice(ZS_IC(1), cur, ZS_IC(0), ZS_IC(0), ZS_IC(PW / 3));
   }
+#undef ZS_IC
   tile_wait_barrier<0>();
   // for acc_get: every MFMA is in front of these statements, and its 16 passes
   // and the read's wait states behind the last

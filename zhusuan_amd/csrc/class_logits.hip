@@ -492,9 +492,9 @@ int launch_tile(const ClassArgs& a, hipStream_t s) {
   return ZSHMC_OK;
 }
 
-template <bool AK, bool BK> using Big = TileCfg<MmaBf16, 2, 2, 4, 4, AK, BK, 2>;
-template <bool AK, bool BK> using Mid = TileCfg<MmaBf16, 2, 2, 2, 2, AK, BK, 2>;
-using Few = TileCfg<MmaBf16, 4, 1, 1, 1, false, false, 3>;
+template <bool AK, bool BK> using Big = TileCfg<MmaBf16, 2, 2, 4, 4, AK, BK>;
+template <bool AK, bool BK> using Mid = TileCfg<MmaBf16, 2, 2, 2, 2, AK, BK>;
+using Few = TileCfg<MmaBf16, 4, 1, 1, 1, false, false>;
 
 template <int EPI, bool F32>
 int launch_logits(const ClassArgs& a, int tile, hipStream_t s) {

@@ -267,9 +267,9 @@ int launch_int8(const Int8Args& a, hipStream_t s) {
   return ZSHMC_OK;
 }
 
-using BigI8 = TileCfg<MmaI8, 2, 2, 4, 4, false, false, 2>;
-using MidI8 = TileCfg<MmaI8, 2, 2, 2, 2, false, false, 2>;
-using FewI8 = TileCfg<MmaI8, 1, 4, 1, 1, false, false, 3>;
+using BigI8 = TileCfg<MmaI8, 2, 2, 4, 4, false, false>;
+using MidI8 = TileCfg<MmaI8, 2, 2, 2, 2, false, false>;
+using FewI8 = TileCfg<MmaI8, 1, 4, 1, 1, false, false>;
 
 unsigned rows_grid(int64_t rows) {
   const int64_t b = (rows + 3) / 4;

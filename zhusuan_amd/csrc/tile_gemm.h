@@ -105,6 +105,12 @@ template <typename F, int... I>
 __device__ __forceinline__ void tile_for_impl(F&& f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
 }
+// a value that is the same in every lane, in scalar registers
+__device__ __forceinline__ uint64_t tile_uniform(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (uint64_t)hi << 32 | lo;
+}
 // f(0), ..., f(N - 1) with the index a constant
 template <int N, typename F>
 __device__ __forceinline__ void tile_for(F&& f) {
@@ -112,15 +118,13 @@ __device__ __forceinline__ void tile_for(F&& f) {
 }
 
 // WGM x WGN waves (four), each WM x WN blocks of 32 x 32
-template <typename MMA_, int WGM_, int WGN_, int WM_, int WN_, bool A_KM_, bool B_KM_,
-          int NBUF_>
+template <typename MMA_, int WGM_, int WGN_, int WM_, int WN_, bool A_KM_, bool B_KM_>
 struct TileCfg {
   typedef MMA_ MMA;
-  static constexpr int WGM = WGM_, WGN = WGN_, WM = WM_, WN = WN_, NBUF = NBUF_;
+  static constexpr int WGM = WGM_, WGN = WGN_, WM = WM_, WN = WN_;
   static constexpr bool A_KM = A_KM_, B_KM = B_KM_;
   static constexpr int BM = WGM * WM * 32, BN = WGN * WN * 32;
-  static constexpr int kStage = (BM + BN) * 128;
-  static constexpr int kLds = NBUF * kStage;
+  static constexpr int kLds = (3 * BM + 2 * BN) * 128;
   static_assert(WGM * WGN == 4, "four waves");
   static_assert(!A_KM || BM == 128 || BM == 256, "whole rows per DMA piece");
   static_assert(!B_KM || BN == 128 || BN == 256, "whole rows per DMA piece");
@@ -134,18 +138,23 @@ struct TileSide {
   uint32_t voff[kPieces];
   uint32_t chunk16;          // kc: the lane's chunk offset within 128 bytes
   uint32_t frag[KM ? NB : 4];
-  int64_t step_bytes;
-  const unsigned char* base;
-  int64_t pitch, plane, rows_left, bytes_left;
   tu4 srd;                   // the step that dma() fetches
-  bool cut;                  // ... ends inside its 128 bytes, at byte `left`
-  uint32_t left;
+  // The step after it: where it starts, the bytes from there to the end of what
+  // the tile may touch, the bytes of k left in a row (kc), how many steps have
+  // been aimed at and how many of them in this plane, and the buffer it goes to
+  uint64_t ptr;
+  int64_t remain, step_bytes;
+  int left, issued, ik;
+  uint32_t planes, buf;
+  // ... and what a new plane starts from
+  uint64_t ptr0;
+  int64_t remain0, plane;
 
   // row0: first m (n) of the tile; k0: first step
   __device__ __forceinline__ void init(const TileOperand& o, int64_t row0, int k0,
-                                       int lane, int wave, int blk0) {
-    pitch = o.pitch;
-    plane = o.plane;
+                                       int lane, int wave, int blk0, uint32_t planes_) {
+    const int64_t pitch = o.pitch;
+    int64_t at, end;           // of the first step; of the tile's rows
     if constexpr (!KM) {
       const int sub = lane >> 3;
       const int f = (4 * (wave & 1) + (sub >> 1)) & 7;
@@ -153,9 +162,9 @@ struct TileSide {
 #pragma unroll
       for (int j = 0; j < kPieces; ++j)
         voff[j] = (uint32_t)((8 * (wave + 4 * j) + sub) * pitch) + chunk16;
-      base = o.base + row0 * pitch + (int64_t)k0 * 128;
-      rows_left = o.rows - row0 < ROWS ? o.rows - row0 : ROWS;
-      bytes_left = o.row_bytes - (int64_t)k0 * 128;
+      at = row0 * pitch + (int64_t)k0 * 128;
+      end = ((o.rows - row0 < ROWS ? o.rows : row0 + ROWS) - 1) * pitch + o.row_bytes;
+      left = (int)(o.row_bytes - (int64_t)k0 * 128);
       step_bytes = 128;
       const uint32_t r = OFF + (blk0 * 32 + (lane & 31)) * 128;
 #pragma unroll
@@ -171,9 +180,9 @@ struct TileSide {
 #pragma unroll
       for (int j = 0; j < kPieces; ++j)
         voff[j] = (uint32_t)((RP * (wave + 4 * j) + sub) * pitch) + c * 16;
-      base = o.base + (int64_t)k0 * 64 * pitch + row0 * 2;
-      rows_left = o.rows - (int64_t)k0 * 64;
-      bytes_left = o.row_bytes - row0 * 2;
+      at = (int64_t)k0 * 64 * pitch + row0 * 2;
+      end = (o.rows - 1) * pitch + o.row_bytes;
+      left = 0;
       step_bytes = 64 * pitch;
       const int k3 = (lane & 15) >> 2;
       const uint32_t kr = OFF + (uint32_t)(((lane >> 5) * 8 + k3) * (ROWS * 2)) + (lane & 1) * 8;
@@ -183,33 +192,50 @@ struct TileSide {
         frag[b] = kr + (uint32_t)((ch ^ (4 * k3)) * 16);
       }
     }
-  }
-  // step `ks` (counted from init's k0) of plane `pl` next; nothing if not `live`
-  __device__ __forceinline__ void aim(int pl, int ks, bool live) {
-    const unsigned char* p = base + pl * plane + ks * step_bytes;
-    int64_t n;
-    cut = false;
-    left = 128;
-    if constexpr (!KM) {
-      const int64_t l = bytes_left - (int64_t)ks * 128;
-      n = (rows_left - 1) * pitch + l;
-      cut = l < 128;
-      left = (uint32_t)l;
-    } else {
-      const int64_t r = rows_left - (int64_t)ks * 64;
-      n = ((r < 64 ? r : 64) - 1) * pitch + bytes_left;
-    }
-    const uint64_t a = reinterpret_cast<uint64_t>(p);
-    srd[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
-    srd[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
-    srd[2] = __builtin_amdgcn_readfirstlane(live ? (uint32_t)n : 0u);
+    plane = o.plane;
+    planes = planes_;
+    ptr0 = tile_uniform(reinterpret_cast<uint64_t>(o.base) + (uint64_t)at);
+    remain0 = (int64_t)tile_uniform((uint64_t)(end - at));
+    ptr = ptr0 + (planes & 3) * plane;
+    remain = remain0;
+    issued = ik = 0;
+    buf = 0;
     srd[3] = 0x00020000u;
   }
-  // its j-th piece of this wave
+  // The next step, into the next of `bufs` buffers (returned); an empty
+  // descriptor behind the last one.  A handful of scalar instructions: they sit
+  // between MFMAs, and what does not fit under one delays the next.
+  template <int BUFS>
+  __device__ __forceinline__ uint32_t aim(int steps, int total) {
+    srd[0] = (uint32_t)ptr;
+    srd[1] = (uint32_t)(ptr >> 32);
+    srd[2] = issued < total ? (remain >> 32 ? 0xffffffffu : (uint32_t)remain) : 0u;
+    if constexpr (!KM) {
+      // the last step of an operand whose rows end inside it (never one of
+      // several planes: those are padded)
+      if (left < 128) {
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) voff[j] = chunk16 >= (uint32_t)left ? 0xffffff00u : voff[j];
+      }
+      left -= 128;
+    }
+    ptr += step_bytes;
+    remain -= step_bytes;
+    ++issued;
+    if (++ik == steps) {
+      ik = 0;
+      planes >>= 2;
+      ptr = ptr0 + (planes & 3) * plane;
+      remain = remain0;
+      if constexpr (!KM) left += steps * 128;
+    }
+    const uint32_t dst = buf * (ROWS * 128);
+    if (++buf == BUFS) buf = 0;
+    return dst;
+  }
+  // its j-th piece of this wave, into the buffer at `lds` (the operand's first)
   __device__ __forceinline__ void dma(int j, uint32_t lds, int wave) const {
-    uint32_t v = voff[j];
-    if constexpr (!KM) v = cut && chunk16 >= left ? 0xffffff00u : v;
-    tile_dma16(srd, v, lds + (uint32_t)(OFF + (wave + 4 * j) * 1024));
+    tile_dma16(srd, voff[j], lds + (uint32_t)(OFF + (wave + 4 * j) * 1024));
   }
   // block b's fragment of slice kk
   __device__ __forceinline__ void read(tu4& f, uint32_t stage, int kk, int b) const {
@@ -237,42 +263,29 @@ __device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperan
                                           uint32_t lds, int lane, int wave,
                                           typename C::MMA::Acc (&acc)[C::WM][C::WN]) {
   typedef TileSide<C::A_KM, C::BM, 0, C::WM> SideA;
-  typedef TileSide<C::B_KM, C::BN, C::BM * 128, C::WN> SideB;
-  constexpr int PA = SideA::kPieces, PW = PA + SideB::kPieces;
-  constexpr int NBUF = C::NBUF, M = C::WM * C::WN, R = C::WM + C::WN;
+  typedef TileSide<C::B_KM, C::BN, 3 * C::BM * 128, C::WN> SideB;
+  constexpr int PA = SideA::kPieces, PB = SideB::kPieces;
+  constexpr int M = C::WM * C::WN, R = C::WM + C::WN;
   SideA sa;
   SideB sb;
-  sa.init(A, m0, k0, lane, wave, (wave / C::WGN) * C::WM);
-  sb.init(B, n0, k0, lane, wave, (wave % C::WGN) * C::WN);
+  sa.init(A, m0, k0, lane, wave, (wave / C::WGN) * C::WM, terms > 1 ? kTermsA3 : 0u);
+  sb.init(B, n0, k0, lane, wave, (wave % C::WGN) * C::WN, terms > 1 ? kTermsB3 : 0u);
 #pragma unroll
   for (int i = 0; i < C::WM; ++i)
 #pragma unroll
     for (int j = 0; j < C::WN; ++j) acc[i][j] = typename C::MMA::Acc{};
 
   const int total = terms * steps;
-  const uint32_t ta = terms > 1 ? kTermsA3 : 0u, tb = terms > 1 ? kTermsB3 : 0u;
-  // the next step to issue: its term, k-step and buffer
-  int issued = 0, it = 0, ik = 0, ibuf = 0;
-  uint32_t dst = lds;
-  auto aim = [&]() {
-    const bool live = issued < total;
-    sa.aim((ta >> (2 * it)) & 3, ik, live);
-    sb.aim((tb >> (2 * it)) & 3, ik, live);
-    dst = lds + (uint32_t)(ibuf * C::kStage);
-    ++issued;
-    if (++ik == steps) ik = 0, ++it;
-    if (++ibuf == NBUF) ibuf = 0;
-  };
-  auto dma = [&](int j) {
-    if (j < PA)
-      sa.dma(j, dst, wave);
-    else
-      sb.dma(j - PA, dst, wave);
-  };
+  uint32_t adst = lds, bdst = lds;
+  auto aim_a = [&]() { adst = lds + sa.template aim<3>(steps, total); };
+  auto aim_b = [&]() { bdst = lds + sb.template aim<2>(steps, total); };
+  auto aim_none = []() {};
   tu4 fa[2][C::WM], fb[2][C::WN];
-  // The MFMAs of register set S, in between the reads of slice KK_ of `stage`
-  // into the other set and the pieces [D0, D1) of the step aimed at
-  auto slice = [&](auto S, uint32_t stage, auto KK, auto D0, auto D1) {
+  // The MFMAs of register set S, in between the reads of slice KK into the other
+  // set and the pieces [D0, D1) of the step that A (B) is aimed at
+  uint32_t acur = lds, bcur = lds;
+  // `then`: what is aimed at next, under the slice's last MFMAs
+  auto slice = [&](auto S, auto KK, auto IS_A, auto D0, auto D1, auto&& then) {
     constexpr int s = decltype(S)::value, kk = decltype(KK)::value;
     constexpr int d0 = decltype(D0)::value, nd = decltype(D1)::value - d0;
     tile_for<M>([&](auto M_) {
@@ -281,16 +294,22 @@ __device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperan
         constexpr int q = decltype(Q)::value;
         if constexpr (q * M / R == m) {
           if constexpr (q < C::WN)
-            sb.read(fb[s ^ 1][q], stage, kk, q);
+            sb.read(fb[s ^ 1][q], bcur, kk, q);
           else
-            sa.read(fa[s ^ 1][q - C::WN], stage, kk, q - C::WN);
+            sa.read(fa[s ^ 1][q - C::WN], acur, kk, q - C::WN);
         }
       });
       tile_for<nd>([&](auto Q) {
         constexpr int q = decltype(Q)::value;
-        if constexpr (q * M / nd == m) dma(d0 + q);
+        if constexpr (q * M / nd == m) {
+          if constexpr (decltype(IS_A)::value)
+            sa.dma(d0 + q, adst, wave);
+          else
+            sb.dma(d0 + q, bdst, wave);
+        }
       });
       constexpr int i = m / C::WN, j = m % C::WN;
+      if constexpr (m == M - 1) then();
       if constexpr (m == 0) __builtin_amdgcn_s_setprio(1);
       acc[i][j] = C::MMA::mma(fa[s][i], fb[s][j], acc[i][j]);
       if constexpr (m == M - 1) __builtin_amdgcn_s_setprio(0);
@@ -298,27 +317,36 @@ __device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperan
     });
   };
 #define ZS_IC(x) std::integral_constant<int, (x)>{}
-  for (int t = 0; t < NBUF; ++t) {
-    aim();
+  aim_a();
 #pragma unroll
-    for (int j = 0; j < PW; ++j) dma(j);
-  }
-  tile_wait_barrier<(NBUF - 1) * PW>();
-  uint32_t cur = lds;
-  tile_for<C::WN>([&](auto Q) { sb.read(fb[0][decltype(Q)::value], cur, 0, decltype(Q)::value); });
-  tile_for<C::WM>([&](auto Q) { sa.read(fa[0][decltype(Q)::value], cur, 0, decltype(Q)::value); });
-  int buf = 0;
+  for (int j = 0; j < PA; ++j) sa.dma(j, adst, wave);
+  aim_b();
+#pragma unroll
+  for (int j = 0; j < PB; ++j) sb.dma(j, bdst, wave);
+  aim_a();
+#pragma unroll
+  for (int j = 0; j < PA; ++j) sa.dma(j, adst, wave);
+  aim_b();
+#pragma unroll
+  for (int j = 0; j < PB / 2; ++j) sb.dma(j, bdst, wave);
+  tile_wait_barrier<PA + PB / 2>();
+  tile_for<C::WN>([&](auto Q) { sb.read(fb[0][decltype(Q)::value], bcur, 0, decltype(Q)::value); });
+  tile_for<C::WM>([&](auto Q) { sa.read(fa[0][decltype(Q)::value], acur, 0, decltype(Q)::value); });
+  uint32_t abuf = 0;
   for (int t = 0; t < total; ++t) {
-    slice(ZS_IC(0), cur, ZS_IC(1), ZS_IC(PW / 3), ZS_IC(PW * 2 / 3));
-    slice(ZS_IC(1), cur, ZS_IC(2), ZS_IC(PW * 2 / 3), ZS_IC(PW));
-    slice(ZS_IC(0), cur, ZS_IC(3), ZS_IC(0), ZS_IC(0));
-    // step t + 1 has landed (those behind it may be in flight), and every wave
-    // has its last slice of step t in registers: its buffer is free
-    tile_wait_barrier<(NBUF - 2) * PW>();
-    if (++buf == NBUF) buf = 0;
-    cur = lds + (uint32_t)(buf * C::kStage);
-    aim();
-    slice(ZS_IC(1), cur, ZS_IC(0), ZS_IC(0), ZS_IC(PW / 3));
+    // B of step t + 1
+    slice(ZS_IC(0), ZS_IC(1), ZS_IC(0), ZS_IC(PB / 2), ZS_IC(PB), aim_a);
+    // A of step t + 2
+    slice(ZS_IC(1), ZS_IC(2), ZS_IC(1), ZS_IC(0), ZS_IC(PA / 2), aim_none);
+    slice(ZS_IC(0), ZS_IC(3), ZS_IC(1), ZS_IC(PA / 2), ZS_IC(PA), aim_b);
+    // step t + 1 has landed (A of step t + 2 may be in flight), and every wave
+    // has its last slice of step t in registers: its buffers are free
+    tile_wait_barrier<PA>();
+    if (++abuf == 3) abuf = 0;
+    acur = lds + abuf * (C::BM * 128);
+    bcur = lds + ((t + 1) & 1) * (C::BN * 128);
+    // B of step t + 2
+    slice(ZS_IC(1), ZS_IC(0), ZS_IC(0), ZS_IC(0), ZS_IC(PB / 2), aim_none);
   }
 #undef ZS_IC
   tile_wait_barrier<0>();

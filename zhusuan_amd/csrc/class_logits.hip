@@ -73,6 +73,13 @@ __global__ void pack_rows_kernel(const void* __restrict__ src, int64_t rows, int
   }
 }
 
+// (maximum, sum of exponentials) of two sets of classes together
+__device__ __forceinline__ cf2 join(const cf2& t, const cf2& u) {
+  const float mx = fmaxf(t[0], u[0]);
+  const float off = mx == -__builtin_inff() ? 0.f : mx;
+  return cf2{mx, t[1] * fast_exp(t[0] - off) + u[1] * fast_exp(u[0] - off)};
+}
+
 // ---- the tile kernels ----------------------------------------------------------
 enum { kEpiStats, kEpiResidual, kEpiStore };
 
@@ -95,18 +102,18 @@ struct ClassArgs {
   int64_t resid_pitch, resid_plane;
   float* bias_part;                // [tiles_n][bias_ld], or NULL
   int64_t bias_ld;
-  // kEpiStore
+  // kEpiStore: out[n, m]
   void* out;
   int64_t out_ld, out_split;       // elements; split s at out + s * out_split
   int out_bf16, accumulate;
 };
 
-// LDS that the epilogue's exchange takes (the biases and their column sums sit
-// behind it)
+// LDS behind the tile loop: what the epilogue exchanges; behind that the tile's
+// biases and their gradient's column sums
 template <typename C, int EPI>
-constexpr int kEpiLds = EPI == kEpiResidual ? C::BN * (C::BM * 2 + 16)
-                        : EPI == kEpiStats  ? C::WGM * C::BN * 8
-                                            : 0;
+constexpr int kEpiLds = EPI == kEpiStats    ? C::WGM * C::BN * 8
+                        : EPI == kEpiResidual ? kTileRowsLds<C, uint16_t>
+                                              : kTileRowsLds<C, float>;
 
 template <typename C, int EPI, bool F32>
 __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_kernel(
@@ -125,6 +132,42 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
     k0 = (int)blockIdx.y * per;
     steps = p.steps - k0 < per ? p.steps - k0 : per;
   }
+  const int wm = wave / C::WGN, wn = wave % C::WGN;
+  const int half = lane >> 5, col = lane & 31;
+  const int mw = wm * C::WM * 32, nw = wn * C::WN * 32;
+
+  // What the epilogue needs of its rows of X (a lane each per block column),
+  // fetched in front of the loop: the label's class counted from the wave's
+  // first (or -1), M, g and -g / S
+  int yl[C::WN];
+  float mx[C::WN], g[C::WN], ginv[C::WN], bias_here = 0.f;
+  const bool biased = EPI != kEpiStore && (p.bias || m0 + C::BM > p.m);
+  if constexpr (EPI != kEpiStore) {
+#pragma unroll
+    for (int j = 0; j < C::WN; ++j) {
+      const int64_t n = n0 + nw + j * 32 + col;
+      yl[j] = -1;
+      // (a row behind the last one, or one that is ignored: r = 0 * e^-inf)
+      mx[j] = 3e38f;
+      g[j] = ginv[j] = 0.f;
+      if (n < p.n) {
+        const int64_t label = p.labels[n];
+        const int64_t y = label - p.class0 - m0 - mw;
+        if (y >= 0 && y < C::WM * 32 && y + m0 + mw < p.m) yl[j] = (int)y;
+        if (EPI == kEpiResidual && !(p.has_ignore && label == p.ignore)) {
+          const cf2 st = p.stats[n];
+          mx[j] = st[0];
+          g[j] = label < 0 || label >= p.n_classes ? __builtin_nanf("") : p.g[n];
+          ginv[j] = -g[j] / st[1];
+        }
+      }
+    }
+    // thread t: the bias of the tile's class t, -inf behind the last class
+    const int64_t v = m0 + threadIdx.x;
+    if (threadIdx.x < C::BM)
+      bias_here = v < p.m ? (p.bias ? p.bias[v] : 0.f) : -__builtin_inff();
+  }
+
   typename C::MMA::Acc acc[C::WM][C::WN];
   if (steps > 0) {
     tile_loop<C>(p.a, p.b, m0, n0, k0, steps, p.terms, lds, lane, wave, acc);
@@ -135,181 +178,156 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
       for (int j = 0; j < C::WN; ++j) acc[i][j] = typename C::MMA::Acc{};
   }
 
-  const int wm = wave / C::WGN, wn = wave % C::WGN;
-  const int half = lane >> 5, col = lane & 31;
-  const int mw = wm * C::WM * 32, nw = wn * C::WN * 32;
-
   if constexpr (EPI == kEpiStore) {
-    const int64_t at = (int64_t)blockIdx.y * p.out_split + (m0 + mw) * p.out_ld + n0 + nw;
-    const int ld = (int)p.out_ld;
-    const int rows = p.m - m0 - mw < C::BM ? (int)(p.m - m0 - mw) : C::BM;
-    const int cols = p.n - n0 - nw < C::BN ? (int)(p.n - n0 - nw) : C::BN;
+    auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < C::WM; ++i)
+      for (int r = 0; r < 4; ++r)
+        v[r] = acc_get(acc[decltype(I)::value][decltype(J)::value], 4 * decltype(Q)::value + r);
+    };
+    if (p.out_bf16) {
+      tile_rows<C, uint16_t>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+        if (n0 + n < p.n && m0 + m < p.m)
+          store_piece(static_cast<uint16_t*>(p.out) + (n0 + n) * p.out_ld + m0 + m,
+                      p.m - m0 - m, piece);
+      });
+    } else {
+      float* out = static_cast<float*>(p.out) + (int64_t)blockIdx.y * p.out_split;
+      tile_rows<C, float>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+        if (n0 + n >= p.n || m0 + m >= p.m) return;
+        float* o = out + (n0 + n) * p.out_ld + m0 + m;
+        tu4 sum = piece;
+        if (p.accumulate) {
 #pragma unroll
-      for (int j = 0; j < C::WN; ++j) {
-        const int c = j * 32 + col;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int m = i * 32 + acc_row(r, half);
-          const float v = acc_get(acc[i][j], r);
-          if (m >= rows || c >= cols) continue;
-          const int o = m * ld + c;
-          if (p.out_bf16) {
-            (static_cast<uint16_t*>(p.out) + at)[o] = bf16_bits(v);
-          } else {
-            float* q = static_cast<float*>(p.out) + at + o;
-            *q = p.accumulate ? *q + v : v;
-          }
+          for (int e = 0; e < 4; ++e)
+            if (e < p.m - m0 - m) {
+              const uint32_t u = piece[e];
+              sum[e] = __builtin_bit_cast(uint32_t, o[e] + __builtin_bit_cast(float, u));
+            }
         }
-      }
+        store_piece(o, p.m - m0 - m, sum);
+      });
+    }
     return;
   } else {
-    // the tile's biases, -inf behind the last class; they stay in the LDS
-    // beside what follows
     float* sbias = reinterpret_cast<float*>(smem + kEpiLds<C, EPI>);
-    for (int i = threadIdx.x; i < C::BM; i += 256) {
-      const int64_t v = m0 + i;
-      sbias[i] = v < p.m ? (p.bias ? p.bias[v] : 0.f) : -__builtin_inff();
+    // the lane's 16 WM classes' biases stay in registers (read per use, the LDS'
+    // latency shows between the accumulator reads)
+    tf4 bias[C::WM][4] = {};
+    if (biased) {
+      if (threadIdx.x < C::BM) sbias[threadIdx.x] = bias_here;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::WM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          bias[i][q] = *reinterpret_cast<const tf4*>(sbias + mw + 4 * half + i * 32 + 8 * q);
     }
-    __syncthreads();
-    const float* sb = sbias + mw + 4 * half;
+    // the logits of registers 4 q .. 4 q + 3 of block (i, j)
+    auto logits = [&](auto I, auto J, auto Q, float (&l)[4]) {
+      constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) l[r] = acc_get(acc[i][j], 4 * q + r) + bias[i][q][r];
+    };
+    auto blocks = [&](auto&& f) {
+      tile_for<C::WM>([&](auto I) { tile_for<4>([&](auto Q) { f(I, Q); }); });
+    };
     if constexpr (EPI == kEpiStats) {
       cf2* red = reinterpret_cast<cf2*>(smem);               // [WGM][BN]
+      tile_for<C::WN>([&](auto J) {
+        constexpr int j = decltype(J)::value;
+        float most = -__builtin_inff();
+        blocks([&](auto I, auto Q) {
+          float l[4];
+          logits(I, J, Q, l);
+          most = fmaxf(fmaxf(most, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
+        });
+        if (__any(yl[j] >= 0)) {           // some row's label is in these classes
+          float picked = 0.f;
+          blocks([&](auto I, auto Q) {
+            constexpr int i = decltype(I)::value, q = decltype(Q)::value;
+            float l[4];
+            logits(I, J, Q, l);
 #pragma unroll
-      for (int j = 0; j < C::WN; ++j) {
-        const int64_t n = n0 + nw + j * 32 + col;
-        int64_t y = -1;
-        if (n < p.n) y = p.labels[n] - m0 - mw;
-        const int yl = y >= 0 && y < C::WM * 32 && y + m0 + mw < p.m ? (int)y : -1;
-        float mx = -__builtin_inff();
-        float picked = 0.f;
+            for (int r = 0; r < 4; ++r)
+              if (yl[j] == i * 32 + acc_row(4 * q + r, half)) picked = l[r];
+          });
+          if (yl[j] >= 0 && ((yl[j] >> 2) & 1) == half)
+            p.label_logit[n0 + nw + j * 32 + col] = picked;
+        }
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const float off = most == -__builtin_inff() ? 0.f : most;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        blocks([&](auto I, auto Q) {
+          float l[4];
+          logits(I, J, Q, l);
 #pragma unroll
-        for (int i = 0; i < C::WM; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const tf4 b = *reinterpret_cast<const tf4*>(sb + i * 32 + 8 * q);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float l = acc_get(acc[i][j], 4 * q + r) + b[r];
-              mx = fmaxf(mx, l);
-              if (yl == i * 32 + acc_row(4 * q + r, half)) picked = l;
-            }
-          }
-        if (yl >= 0 && ((yl >> 2) & 1) == half) p.label_logit[n] = picked;
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float off = mx == -__builtin_inff() ? 0.f : mx;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < C::WM; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const tf4 b = *reinterpret_cast<const tf4*>(sb + i * 32 + 8 * q);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s += fast_exp((acc_get(acc[i][j], 4 * q + r) + b[r]) - off);
-          }
-        s += __shfl_xor(s, 32, 64);
-        if (half == 0) red[wm * C::BN + nw + j * 32 + col] = cf2{mx, s};
-      }
+          for (int r = 0; r < 4; ++r) s[r] += fast_exp(l[r] - off);
+        });
+        float sum = (s[0] + s[1]) + (s[2] + s[3]);
+        sum += __shfl_xor(sum, 32, 64);
+        if (half == 0) red[wm * C::BN + nw + j * 32 + col] = cf2{most, sum};
+      });
       __syncthreads();
       for (int i = threadIdx.x; i < C::BN; i += 256) {
         if (n0 + i >= p.n) continue;
         cf2 t = red[i];
 #pragma unroll
-        for (int k = 1; k < C::WGM; ++k) {
-          const cf2 u = red[k * C::BN + i];
-          const float mx = fmaxf(t[0], u[0]);
-          const float off = mx == -__builtin_inff() ? 0.f : mx;
-          t = cf2{mx, t[1] * fast_exp(t[0] - off) + u[1] * fast_exp(u[0] - off)};
-        }
+        for (int k = 1; k < C::WGM; ++k) t = join(t, red[k * C::BN + i]);
         p.part[(int64_t)tm * p.n + n0 + i] = t;
       }
     } else {
-      // what a row of X (a lane) contributes: g, -g / S, M, its label here
-      float g[C::WN], ginv[C::WN], mx[C::WN];
-      int yl[C::WN];
-      bool zero[C::WN];
-#pragma unroll
-      for (int j = 0; j < C::WN; ++j) {
-        const int64_t n = n0 + nw + j * 32 + col;
-        g[j] = ginv[j] = mx[j] = 0.f;
-        yl[j] = -1;
-        zero[j] = true;
-        if (n < p.n) {
-          const int64_t label = p.labels[n];
-          const cf2 st = p.stats[n];
-          mx[j] = st[0];
-          g[j] = label < 0 || label >= p.n_classes ? __builtin_nanf("") : p.g[n];
-          ginv[j] = -g[j] / st[1];
-          zero[j] = p.has_ignore && label == p.ignore;
-          const int64_t y = label - p.class0 - m0 - mw;
-          if (y >= 0 && y < C::WM * 32) yl[j] = (int)y;
-        }
-      }
-      // The tile goes through LDS ([row of X][class], rows 16 bytes apart modulo
-      // the banks) so that whole lines of r are written, one plane at a time;
-      // the later planes of a float32 r compute it again rather than keep it.
-      constexpr int kPitch = C::BM * 2 + 16;
-      constexpr int kPlanes = F32 ? 3 : 1;
-      constexpr int kChunks = C::BM / 8;
-      float* scol = sbias + C::BM;                           // [WGN][BM]
+      // r, one plane at a time; the later planes of a float32 r compute it
+      // again rather than keep it
+      float sum[C::WM][16];                // over the wave's rows, for the bias
+      float* scol = sbias + C::BM;         // [WGN][BM]
 #pragma unroll 1
-      for (int pl = 0; pl < kPlanes; ++pl) {
-        // (or the compiler keeps every label comparison across the planes)
+      for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) {
+        if (pl) __syncthreads();           // the plane before has been read
+        auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
+          constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
+          logits(I, J, Q, v);
 #pragma unroll
-        for (int j = 0; j < C::WN; ++j) asm volatile("" : "+v"(yl[j]));
+          for (int r = 0; r < 4; ++r) v[r] = ginv[j] * fast_exp(v[r] - mx[j]);
+          if (__any(yl[j] >= 0)) {
 #pragma unroll
-        for (int i = 0; i < C::WM; ++i)
+            for (int r = 0; r < 4; ++r)
+              if (yl[j] == i * 32 + acc_row(4 * q + r, half)) v[r] += g[j];
+          }
+          if (pl == 0 && p.bias_part) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const tf4 b = *reinterpret_cast<const tf4*>(sb + i * 32 + 8 * q);
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
+          }
+          if (F32) {
 #pragma unroll
-            for (int j = 0; j < C::WN; ++j) {
-              uint16_t h[4];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                // (behind the last class l = -inf and r = 0; where the row's own r
-                // is NaN, so is everything that those columns reach)
-                const float l = acc_get(acc[i][j], 4 * q + r) + b[r];
-                const float hit = yl[j] == i * 32 + acc_row(4 * q + r, half) ? g[j] : 0.f;
-                float v = hit + ginv[j] * fast_exp(l - mx[j]);
-                v = zero[j] ? 0.f : v;
-                if (pl == 0) sum[r] += v;
-                if (F32) {
-                  const float v1 = v - bf16_value(bf16_bits(v));
-                  v = pl == 0 ? v : pl == 1 ? v1 : v1 - bf16_value(bf16_bits(v1));
-                }
-                h[r] = bf16_bits(v);
-              }
-              *reinterpret_cast<tu2*>(smem + (nw + j * 32 + col) * kPitch +
-                                      (mw + i * 32 + 8 * q + 4 * half) * 2) =
-                  tu2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
-            }
-            if (pl == 0 && p.bias_part) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float s = group_sum<32>(sum[r]);
-                if (col == 0) scol[wn * C::BM + mw + i * 32 + acc_row(4 * q + r, half)] = s;
-              }
+            for (int r = 0; r < 4; ++r) {
+              const float v1 = v[r] - bf16_value(bf16_bits(v[r]));
+              v[r] = pl == 0 ? v[r] : pl == 1 ? v1 : v1 - bf16_value(bf16_bits(v1));
             }
           }
-        __syncthreads();
-        for (int c = threadIdx.x; c < C::BN * kChunks; c += 256) {
-          const int row = c / kChunks, ch = c % kChunks;
-          const int64_t n = n0 + row, byte = (m0 + ch * 8) * 2;
-          if (n < p.n && byte < p.resid_pitch)
-            *reinterpret_cast<tu4*>(p.resid + pl * p.resid_plane + n * p.resid_pitch + byte) =
-                *reinterpret_cast<const tu4*>(smem + row * kPitch + ch * 16);
-        }
-        if (pl == 0 && p.bias_part)
+        };
+        tile_rows<C, uint16_t>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+          const int64_t byte = (m0 + m) * 2;
+          if (n0 + n < p.n && byte < p.resid_pitch)
+            *reinterpret_cast<tu4*>(p.resid + pl * p.resid_plane + (n0 + n) * p.resid_pitch +
+                                    byte) = piece;
+        });
+        if (pl == 0 && p.bias_part) {
+          blocks([&](auto I, auto Q) {
+            constexpr int i = decltype(I)::value, q = decltype(Q)::value;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float s = group_sum<32>(sum[i][4 * q + r]);
+              if (col == 0) scol[wn * C::BM + mw + i * 32 + acc_row(4 * q + r, half)] = s;
+            }
+          });
+          __syncthreads();
           for (int i = threadIdx.x; i < C::BM; i += 256) {
             float s = 0.f;
 #pragma unroll
             for (int k = 0; k < C::WGN; ++k) s += scol[k * C::BM + i];
             if (m0 + i < p.m) p.bias_part[(int64_t)tn * p.bias_ld + p.class0 + m0 + i] = s;
           }
-        if (pl + 1 < kPlanes) __syncthreads();
+        }
       }
     }
   }
@@ -323,25 +341,14 @@ __global__ __launch_bounds__(256) void join_stats_kernel(
     int64_t ignore, float* __restrict__ log_prob, cf2* __restrict__ stats) {
   const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
   const int k = threadIdx.x >> 4;
-  const float ninf = -__builtin_inff();
-  cf2 t{ninf, 0.f};
+  cf2 t{-__builtin_inff(), 0.f};
   if (row < n)
-    for (int i = k; i < parts; i += 16) {
-      const cf2 u = part[(int64_t)i * n + row];
-      const float mx = fmaxf(t[0], u[0]);
-      const float off = mx == ninf ? 0.f : mx;
-      t = cf2{mx, t[1] * fast_exp(t[0] - off) + u[1] * fast_exp(u[0] - off)};
-    }
+    for (int i = k; i < parts; i += 16) t = join(t, part[(int64_t)i * n + row]);
   __shared__ cf2 s[16][16];
   s[k][threadIdx.x & 15] = t;
   __syncthreads();
   if (k || row >= n) return;
-  for (int i = 1; i < 16; ++i) {
-    const cf2 u = s[i][threadIdx.x & 15];
-    const float mx = fmaxf(t[0], u[0]);
-    const float off = mx == ninf ? 0.f : mx;
-    t = cf2{mx, t[1] * fast_exp(t[0] - off) + u[1] * fast_exp(u[0] - off)};
-  }
+  for (int i = 1; i < 16; ++i) t = join(t, s[i][threadIdx.x & 15]);
   const int64_t y = labels[row];
   float lp = __builtin_nanf("");
   if (has_ignore && y == ignore)
@@ -674,10 +681,10 @@ extern "C" int zshmc_class_log_prob_grad(
     if (rc != ZSHMC_OK) return rc;
     if (grad_w) {                  // dw = r^T X over the rows of X
       ClassArgs g{};
-      g.a = r;
-      g.b = ox;
-      g.m = c;
-      g.n = q.d;
+      g.a = ox;
+      g.b = r;
+      g.m = q.d;
+      g.n = c;
       g.steps = (int)tiles(q.n, 64);
       g.terms = terms;
       g.splits = 1;
@@ -690,10 +697,10 @@ extern "C" int zshmc_class_log_prob_grad(
     }
     if (grad_x) {                  // dX += r w over the piece's classes
       ClassArgs g{};
-      g.a = r;
-      g.b = wp;
-      g.m = q.n;
-      g.n = q.d;
+      g.a = wp;
+      g.b = r;
+      g.m = q.d;
+      g.n = q.n;
       g.steps = (int)tiles(c, 64);
       g.terms = terms;
       g.splits = l.dx_splits;
@@ -701,8 +708,8 @@ extern "C" int zshmc_class_log_prob_grad(
       g.out_ld = q.d;
       g.out_split = q.n * q.d;
       g.accumulate = c0 > 0;
-      rc = l.dx_tile == 0 ? launch_tile<Big<false, true>, kEpiStore, false>(g, s)
-                          : launch_tile<Mid<false, true>, kEpiStore, false>(g, s);
+      rc = l.dx_tile == 0 ? launch_tile<Big<true, false>, kEpiStore, false>(g, s)
+                          : launch_tile<Mid<true, false>, kEpiStore, false>(g, s);
       if (rc != ZSHMC_OK) return rc;
     }
   }

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(
 
 // ---- the product ------------------------------------------------------------------
 struct Int8Args {
-  TileOperand a, b;                // rows of x, channels of w
+  TileOperand a, b;                // channels of w, rows of x
   int64_t m, n;
   int steps;
   uint32_t tiles_m, tiles_n;
@@ -210,50 +210,62 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void int8_tile_ke
   int tm, tn;
   tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
   const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
-  ti16 acc[C::WM][C::WN];
-  tile_loop<C>(p.a, p.b, m0, n0, 0, p.steps, 1, lds, lane, wave, acc);
+  // channel t's scale and bias at thread t, a row's scale at its lane
   const int half = lane >> 5, col = lane & 31;
-  const int64_t mw = m0 + (wave / C::WGN) * C::WM * 32, nw = n0 + (wave % C::WGN) * C::WN * 32;
-  const int rows = p.m - mw < C::BM ? (int)(p.m - mw) : C::BM;
-  const int cols = p.n - nw < C::BN ? (int)(p.n - nw) : C::BN;
-  const int64_t at = mw * p.ldo + nw;
-  const int ld = (int)p.ldo;
-  float sw[C::WN], bias[C::WN];
+  const int mw = (wave / C::WGN) * C::WM * 32, nw = (wave % C::WGN) * C::WN * 32;
+  float sx[C::WN], sw_here = 0.f, bias_here = 0.f;
 #pragma unroll
   for (int j = 0; j < C::WN; ++j) {
-    const int c = j * 32 + col;
-    sw[j] = c < cols ? p.sw[nw + c] : 0.f;
-    bias[j] = p.bias && c < cols ? p.bias[nw + c] : 0.f;
+    const int64_t n = n0 + nw + j * 32 + col;
+    sx[j] = n < p.n ? p.sx[n] : 0.f;
   }
+  if (threadIdx.x < C::BM && m0 + threadIdx.x < p.m) {
+    sw_here = p.sw[m0 + threadIdx.x];
+    if (p.bias) bias_here = p.bias[m0 + threadIdx.x];
+  }
+  ti16 acc[C::WM][C::WN];
+  tile_loop<C>(p.a, p.b, m0, n0, 0, p.steps, 1, lds, lane, wave, acc);
+  typedef typename std::conditional<BF16, uint16_t, float>::type T;
+  float* ssw = reinterpret_cast<float*>(smem + kTileRowsLds<C, T>);     // [2][BM]
+  if (threadIdx.x < C::BM) {
+    ssw[threadIdx.x] = sw_here;
+    ssw[C::BM + threadIdx.x] = bias_here;
+  }
+  __syncthreads();
+  tf4 sw[C::WM][4], bias[C::WM][4];
 #pragma unroll
   for (int i = 0; i < C::WM; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int m = i * 32 + acc_row(r, half);
-      const float sx = m < rows ? p.sx[mw + m] : 0.f;
-#pragma unroll
-      for (int j = 0; j < C::WN; ++j) {
-        const int c = j * 32 + col;
-        const float v = (float)acc_get(acc[i][j], r) * (sx * sw[j]) + bias[j];
-        if (m >= rows || c >= cols) continue;
-        const int o = m * ld + c;
-        if (BF16)
-          (static_cast<__bf16*>(p.out) + at)[o] = (__bf16)v;
-        else
-          (static_cast<float*>(p.out) + at)[o] = v;
-      }
+    for (int q = 0; q < 4; ++q) {
+      const float* mine = ssw + mw + 4 * half + i * 32 + 8 * q;
+      sw[i][q] = *reinterpret_cast<const tf4*>(mine);
+      bias[i][q] = *reinterpret_cast<const tf4*>(mine + C::BM);
     }
+  auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
+    constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      v[r] = (float)acc_get(acc[i][j], 4 * q + r) * (sx[j] * sw[i][q][r]) + bias[i][q][r];
+  };
+  tile_rows<C, T>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+    if (n0 + n < p.n && m0 + m < p.m)
+      store_piece(static_cast<T*>(p.out) + (n0 + n) * p.ldo + m0 + m, p.m - m0 - m, piece);
+  });
 }
 
 template <typename C, bool BF16>
 int launch_int8(const Int8Args& a, hipStream_t s) {
+  constexpr int epi =
+      kTileRowsLds<C, typename std::conditional<BF16, uint16_t, float>::type> + C::BM * 8;
+  constexpr int lds = C::kLds > epi ? C::kLds : epi;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
   static thread_local int attr_dev = -1;
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
   if (attr_dev != dev) {
     const hipError_t e = hipFuncSetAttribute(
         reinterpret_cast<const void*>(int8_tile_kernel<C, BF16>),
-        hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(LDS)");
     attr_dev = dev;
   }
@@ -262,14 +274,14 @@ int launch_int8(const Int8Args& a, hipStream_t s) {
   p.tiles_n = (uint32_t)((p.n + C::BN - 1) / C::BN);
   const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n;
   ZS_REQUIRE(wgs < (1ll << 31), "zshmc_int8_linear: %lld tiles", (long long)wgs);
-  hipLaunchKernelGGL((int8_tile_kernel<C, BF16>), dim3((unsigned)wgs), dim3(256), C::kLds, s, p);
+  hipLaunchKernelGGL((int8_tile_kernel<C, BF16>), dim3((unsigned)wgs), dim3(256), lds, s, p);
   ZS_LAUNCH_CHECK("int8_tile_kernel launch");
   return ZSHMC_OK;
 }
 
 using BigI8 = TileCfg<MmaI8, 2, 2, 4, 4, false, false>;
 using MidI8 = TileCfg<MmaI8, 2, 2, 2, 2, false, false>;
-using FewI8 = TileCfg<MmaI8, 1, 4, 1, 1, false, false>;
+using FewI8 = TileCfg<MmaI8, 4, 1, 1, 1, false, false>;
 
 unsigned rows_grid(int64_t rows) {
   const int64_t b = (rows + 3) / 4;
@@ -361,10 +373,10 @@ extern "C" int zshmc_int8_linear(const int8_t* x, int64_t x_pitch, const float* 
   if (n_rows == 0) return ZSHMC_OK;
   ZS_REQUIRE(x && w && x_scale && w_scale && out, "zshmc_int8_linear: null pointer");
   Int8Args a{};
-  a.a = TileOperand{reinterpret_cast<const unsigned char*>(x), x_pitch, 0, n_rows, bytes};
-  a.b = TileOperand{reinterpret_cast<const unsigned char*>(w), w_pitch, 0, n_channels, bytes};
-  a.m = n_rows;
-  a.n = n_channels;
+  a.a = TileOperand{reinterpret_cast<const unsigned char*>(w), w_pitch, 0, n_channels, bytes};
+  a.b = TileOperand{reinterpret_cast<const unsigned char*>(x), x_pitch, 0, n_rows, bytes};
+  a.m = n_channels;
+  a.n = n_rows;
   a.steps = (int)((bytes + 127) / 128);
   a.sx = x_scale;
   a.sw = w_scale;

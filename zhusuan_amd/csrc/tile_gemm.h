@@ -67,6 +67,13 @@ constexpr int kTerms3 = 6;
 constexpr uint32_t kTermsA3 = 1u | 2u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
 constexpr uint32_t kTermsB3 = 1u | 0u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
 
+// two float32 -> bfloat16 (to nearest even) in one register
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  const pair p = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, p);
+}
+
 struct MmaBf16 {
   typedef tf16 Acc;
   static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
@@ -394,6 +401,69 @@ __device__ __forceinline__ int acc_get(const ti16& v, int r) {
   int x;
   asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(v[r]));
   return x;
+}
+
+// The result's rows leave through the LDS.  A lane holds ONE n and, in groups of
+// four registers, runs of four m: the caller picks its operands so that m is
+// the contiguous direction of the output.  Per block column j, the workgroup's
+// WGN x 32 rows of BM values are written as elements T (float, or bfloat16 bits),
+// 16 bytes between rows so that they start in different banks, and read back
+// in 16-byte pieces; two regions alternate, one barrier a block column.
+//   value(i, j, q, v): the four values of registers 4 q .. 4 q + 3 of block (i, j)
+//   emit(n, m, piece): 16 bytes of row n (of the tile) from column m on
+template <typename C, typename T>
+constexpr int kTileRowsLds = 2 * C::WGN * 32 * (C::BM * (int)sizeof(T) + 16);
+
+template <typename C, typename T, typename V, typename E>
+__device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& value, E&& emit) {
+  constexpr int kRows = C::WGN * 32, kPitch = C::BM * (int)sizeof(T) + 16;
+  constexpr int kPer = 16 / (int)sizeof(T), kPieces = C::BM / kPer;
+  const int half = lane >> 5, col = lane & 31;
+  char* const mine = smem + ((wave % C::WGN) * 32 + col) * kPitch +
+                     ((wave / C::WGN) * C::WM * 32 + 4 * half) * (int)sizeof(T);
+  tile_for<C::WN>([&](auto J) {
+    constexpr int j = decltype(J)::value;
+    constexpr int region = (j & 1) * kRows * kPitch;
+    tile_for<C::WM>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      tile_for<4>([&](auto Q) {
+        constexpr int q = decltype(Q)::value;
+        float v[4];
+        value(I, J, Q, v);
+        char* to = mine + region + (i * 32 + 8 * q) * (int)sizeof(T);
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<tf4*>(to) = tf4{v[0], v[1], v[2], v[3]};
+        else
+          *reinterpret_cast<tu2*>(to) = tu2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+      });
+    });
+    __syncthreads();
+    for (int c = threadIdx.x; c < kRows * kPieces; c += 256) {
+      const int row = c / kPieces, piece = c % kPieces;
+      emit((row >> 5) * C::WN * 32 + j * 32 + (row & 31), piece * kPer,
+           *reinterpret_cast<const tu4*>(smem + region + row * kPitch + piece * 16));
+    }
+  });
+}
+
+// `piece` (16 bytes) to out[0 ..], `left` elements of T still inside the row
+template <typename T>
+__device__ __forceinline__ void store_piece(T* out, int64_t left, const tu4& piece) {
+  constexpr int N = 16 / (int)sizeof(T);
+  if (left >= N) {
+    *reinterpret_cast<tu4_any*>(out) = piece;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (e < left) {
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t u = piece[e];
+        out[e] = __builtin_bit_cast(T, u);
+      } else {
+        out[e] = (T)(piece[e / 2] >> (16 * (e & 1)));
+      }
+    }
 }
 
 }  // namespace zshmc

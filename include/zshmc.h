@@ -1080,6 +1080,17 @@ int zshmc_int8_linear(const int8_t* x, int64_t x_pitch, const float* x_scale,
                       const float* bias, int64_t n_rows, int64_t n_features,
                       int64_t n_channels, void* out, int64_t ldo, int dtype,
                       void* stream);
+/* The same with x [n_rows, n_features] of x_dtype, rows ldx elements apart,
+ * rounded to 8 bits a row on the way (zshmc_quantize_rows).  workspace:
+ * n_rows * (n_features rounded up to a multiple of 128, + 4) bytes, 16-byte
+ * aligned. */
+int zshmc_quantized_linear(const void* x, int64_t ldx, int x_dtype,
+                           const int8_t* w, int64_t w_pitch,
+                           const float* w_scale, const float* bias,
+                           int64_t n_rows, int64_t n_features,
+                           int64_t n_channels, void* out, int64_t ldo,
+                           int dtype, void* workspace, int64_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }

@@ -33,7 +33,7 @@ def check(w, X, y, b, g, ignore=None):
 @pytest.mark.parametrize('dtype', BOTH)
 @pytest.mark.parametrize('N,D,V', [
     (1, 1, 1), (1, 64, 128), (2, 7, 3), (5, 8, 257), (31, 64, 300),
-    (32, 130, 129), (33, 128, 500), (65, 200, 1000), (129, 72, 4099),
+    (32, 130, 129), (33, 128, 500), (64, 100, 777), (65, 200, 1000), (129, 72, 4099),
     (100, 128, 12419), (300, 256, 40000), (1021, 784, 1237)])
 def test_log_prob_and_gradients(N, D, V, dtype):
     for bias, ignore in ((False, None), (True, IGNORE)):

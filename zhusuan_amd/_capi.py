@@ -283,6 +283,9 @@ PROTOTYPES = {
     'zshmc_int8_linear': (c_int, [
         _p, c_int64, _p, _p, c_int64, _p, _p, c_int64, c_int64, c_int64, _p,
         c_int64, c_int, _p]),
+    'zshmc_quantized_linear': (c_int, [
+        _p, c_int64, c_int, _p, c_int64, _p, _p, c_int64, c_int64, c_int64,
+        _p, c_int64, c_int, _p, c_int64, _p]),
 }
 
 
@@ -361,3 +364,38 @@ def ptr(t):
 def current_stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def _raw_stream(index):
+    """current_stream() of device `index`, without the Stream object where
+    torch offers that (2 us of a small call)."""
+    import torch
+    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+    return raw(index) if raw is not None else \
+        torch.cuda.current_stream(index).cuda_stream
+
+
+class on_device(object):
+    """`with on_device(device) as stream:` -- calls on tensors of `device`,
+    whichever device is current, on that device's current stream (a handle).
+    Nothing is switched where it is the current one already."""
+
+    __slots__ = ('index', 'back')
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        import torch
+        here = torch.cuda.current_device()
+        index = here if self.index is None else self.index
+        self.back = None
+        if index != here:
+            torch.cuda.set_device(index)
+            self.back = here
+        return _raw_stream(index)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            import torch
+            torch.cuda.set_device(self.back)

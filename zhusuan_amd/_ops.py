@@ -1010,14 +1010,60 @@ def row_dtype(dtype, what):
 def _rows_2d(t):
     """t [..., K] as a matrix whose rows are contiguous (a view where t's
     strides allow one), and its row stride in elements."""
-    t2 = t.detach().reshape(-1, t.shape[-1])
-    if t2.shape[0] > 1:
-        if t2.stride(1) != 1 and t2.shape[1] > 1 or t2.stride(0) < t2.shape[1]:
-            t2 = t2.contiguous()
-        return t2, max(int(t2.stride(0)), int(t2.shape[1]))
-    if t2.shape[1] > 1 and t2.stride(1) != 1:
+    t2 = t.detach()
+    if t2.dim() != 2:
+        t2 = t2.reshape(-1, t.shape[-1])
+    n, K = t2.shape
+    ld, inner = t2.stride()
+    if (K > 1 and inner != 1) or (n > 1 and ld < K):
         t2 = t2.contiguous()
-    return t2, int(t2.shape[1])
+        ld = K
+    return t2, ld if n > 1 else K
+
+
+_class_workspace = {}
+
+
+def _class_workspace_bytes(x2, w2, dims, gradient):
+    """zshmc_class_log_prob_workspace, remembered per shape (and alignment)."""
+    key = dims[:7] + (gradient, x2.data_ptr() & 15, w2.data_ptr() & 15,
+                      x2.device.index)
+    hit = _class_workspace.get(key)
+    if hit is None:
+        import ctypes
+        N, D, V, ldx, ldw, dtype, has_ignore, _ = dims
+        n = ctypes.c_int64(0)
+        _capi.call('zshmc_class_log_prob_workspace', x2.data_ptr(),
+                   w2.data_ptr(), N, D, V, ldx, ldw, dtype, gradient,
+                   has_ignore, ctypes.addressof(n))
+        if len(_class_workspace) > 256:
+            _class_workspace.clear()
+        hit = _class_workspace[key] = max(int(n.value), 16)
+    return hit
+
+
+def _class_log_prob(w2, ldw, x2, ldx, y, b, ignore_label, with_stats):
+    """(log_prob [N], stats or None, the call's sizes) of contiguous-row
+    matrices."""
+    dims = (x2.shape[0], x2.shape[1], w2.shape[0], ldx, ldw,
+            _ROW_DTYPES[w2.dtype], 0 if ignore_label is None else 1,
+            ignore_label or 0)
+    out = torch.empty(dims[0], dtype=_F32, device=x2.device)
+    stats = torch.empty(dims[0], 2, dtype=_F32, device=x2.device) \
+        if with_stats else None
+    with _capi.on_device(x2.device) as stream:
+        n = _class_workspace_bytes(x2, w2, dims, 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=x2.device)
+        _capi.call('zshmc_class_log_prob', x2.data_ptr(), w2.data_ptr(),
+                   _capi.ptr(b), y.data_ptr(), *dims, out.data_ptr(),
+                   _capi.ptr(stats), ws.data_ptr(), n, stream)
+    return out, stats, dims
+
+
+def _float_row(bias):
+    if bias is None or (bias.dtype == _F32 and bias.is_contiguous()):
+        return bias
+    return bias.detach().to(_F32).contiguous()
 
 
 class ClassLogProb(_Function):
@@ -1027,62 +1073,37 @@ class ClassLogProb(_Function):
 
     @staticmethod
     def forward(ctx, w, X, labels, bias, ignore_label):
-        w2, ldw = _rows_2d(w)
-        x2, ldx = _rows_2d(X)
-        b = None if bias is None else bias.detach().to(_F32).contiguous()
-        y = labels.detach().to(torch.int64).contiguous()
-        N, D, V = x2.shape[0], x2.shape[1], w2.shape[0]
-        ctx.dims = (N, D, V, ldx, ldw, row_dtype(w.dtype, 'w'),
-                    0 if ignore_label is None else 1, ignore_label or 0)
-        ctx.shapes = (tuple(w.shape), tuple(X.shape),
-                      None if bias is None else bias.dtype)
-        out = torch.empty(N, dtype=_F32, device=X.device)
-        need = any(ctx.needs_input_grad)
-        stats = torch.empty(N, 2, dtype=_F32, device=X.device) if need \
-            else None
-        with torch.cuda.device(X.device):
-            ws = ClassLogProb._workspace(x2, w2, ctx.dims, 0)
-            _capi.call('zshmc_class_log_prob', x2.data_ptr(), w2.data_ptr(),
-                       _capi.ptr(b), y.data_ptr(), *(ctx.dims + (
-                           out.data_ptr(), _capi.ptr(stats), ws.data_ptr(),
-                           ws.numel(), _capi.current_stream())))
-        if need:
-            ctx.save_for_backward(w, X, y, b, stats)
+        (w2, ldw), (x2, ldx) = _rows_2d(w), _rows_2d(X)
+        b = _float_row(bias)
+        y = labels.to(torch.int64).contiguous()
+        out, stats, ctx.dims = _class_log_prob(w2, ldw, x2, ldx, y, b,
+                                               ignore_label, True)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(w, X, y, b, stats)
         return out
-
-    @staticmethod
-    def _workspace(x2, w2, dims, gradient):
-        import ctypes
-        N, D, V, ldx, ldw, dtype, has_ignore, _ = dims
-        n = ctypes.c_int64(0)
-        _capi.call('zshmc_class_log_prob_workspace', x2.data_ptr(),
-                   w2.data_ptr(), N, D, V, ldx, ldw, dtype, gradient,
-                   has_ignore, ctypes.addressof(n))
-        return torch.empty(max(int(n.value), 16), dtype=torch.uint8,
-                           device=x2.device)
 
     @staticmethod
     def backward(ctx, gout):
         w, X, y, b, stats = ctx.saved_tensors
         (w2, _), (x2, _) = _rows_2d(w), _rows_2d(X)
-        w_shape, x_shape, b_dtype = ctx.shapes
         need_w, need_x, _, need_b = ctx.needs_input_grad[:4]
+        dev = X.device
         g = gout.to(_F32).contiguous()
-        gw = torch.empty(w_shape, dtype=w.dtype, device=w.device) \
+        gw = torch.empty(w.shape, dtype=w.dtype, device=dev) \
             if need_w else None
-        gx = torch.empty(x_shape, dtype=X.dtype, device=X.device) \
+        gx = torch.empty(X.shape, dtype=X.dtype, device=dev) \
             if need_x else None
-        gb = torch.empty(w_shape[0], dtype=_F32, device=w.device) \
+        gb = torch.empty(w.shape[0], dtype=_F32, device=dev) \
             if need_b else None
-        with torch.cuda.device(X.device):
-            ws = ClassLogProb._workspace(x2, w2, ctx.dims, 1)
+        with _capi.on_device(dev) as stream:
+            n = _class_workspace_bytes(x2, w2, ctx.dims, 1)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
             _capi.call('zshmc_class_log_prob_grad', x2.data_ptr(),
-                       w2.data_ptr(), _capi.ptr(b), y.data_ptr(),
-                       *(ctx.dims + (
-                           stats.data_ptr(), g.data_ptr(), _capi.ptr(gx),
-                           _capi.ptr(gw), _capi.ptr(gb), ws.data_ptr(),
-                           ws.numel(), _capi.current_stream())))
-        return (gw, gx, None, gb.to(b_dtype) if need_b else None, None)
+                       w2.data_ptr(), _capi.ptr(b), y.data_ptr(), *ctx.dims,
+                       stats.data_ptr(), g.data_ptr(), _capi.ptr(gx),
+                       _capi.ptr(gw), _capi.ptr(gb), ws.data_ptr(), n, stream)
+        return (gw, gx, None, gb.to(ctx.bias_dtype) if need_b else None,
+                None)
 
 
 def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
@@ -1118,7 +1139,7 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
         raise ValueError("linear_categorical_log_prob: w [V, D] and X [..., D]"
                          " expected, got {} and {}".format(tuple(w.shape),
                                                            tuple(X.shape)))
-    if tuple(labels.shape) != tuple(X.shape[:-1]):
+    if labels.shape != X.shape[:-1]:
         raise ValueError("linear_categorical_log_prob: labels {} for X {}"
                          .format(tuple(labels.shape), tuple(X.shape)))
     if bias is not None:
@@ -1130,14 +1151,25 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
             raise ValueError("linear_categorical_log_prob: bias {} for {} "
                              "classes".format(tuple(bias.shape), w.shape[0]))
     require_device(w, X, labels, bias)
-    if any(t is not None and t.device != X.device for t in (w, labels, bias)):
+    if w.device != X.device or labels.device != X.device or \
+            (bias is not None and bias.device != X.device):
         raise ValueError("linear_categorical_log_prob: all tensors must be on "
                          "one device")
     if ignore_label is not None:
         ignore_label = int(ignore_label)
-    out = ClassLogProb.apply(w, X.reshape(-1, X.shape[-1]),
-                             labels.reshape(-1), bias, ignore_label)
-    return out.reshape(labels.shape)
+    flat = X.dim() == 2
+    x2 = X if flat else X.reshape(-1, X.shape[-1])
+    y = labels if flat else labels.reshape(-1)
+    if torch.is_grad_enabled() and (
+            w.requires_grad or X.requires_grad or
+            (bias is not None and bias.requires_grad)):
+        out = ClassLogProb.apply(w, x2, y, bias, ignore_label)
+    else:
+        (wr, ldw), (xr, ldx) = _rows_2d(w), _rows_2d(x2)
+        out = _class_log_prob(wr, ldw, xr, ldx,
+                              y.to(torch.int64).contiguous(),
+                              _float_row(bias), ignore_label, False)[0]
+    return out if flat else out.reshape(labels.shape)
 
 
 class QuantizedRows(object):
@@ -1153,24 +1185,36 @@ class QuantizedRows(object):
                 values.dtype != torch.int8 or scale.dtype != _F32:
             raise TypeError("QuantizedRows: int8 values and float32 scale "
                             "tensors expected")
-        if values.dim() < 1 or values.shape[-1] == 0 or \
-                tuple(scale.shape) != tuple(values.shape[:-1]):
+        shape = values.shape
+        if len(shape) < 1 or shape[-1] == 0 or scale.shape != shape[:-1]:
             raise ValueError("QuantizedRows: values [..., K] and scale [...] "
                              "expected, got {} and {}".format(
-                                 tuple(values.shape), tuple(scale.shape)))
+                                 tuple(shape), tuple(scale.shape)))
         require_device(values, scale)
         if values.device != scale.device:
             raise ValueError("QuantizedRows: values and scale must be on one "
                              "device")
-        self._shape = values.shape
-        K = int(values.shape[-1])
-        rows = values.reshape(-1, K)
+        K = int(shape[-1])
+        rows = values if len(shape) == 2 else values.reshape(-1, K)
         if not self._usable(rows):
             rows = self._padded(rows)
-        self._rows, self.scale = rows, scale
-        self._flat_scale = scale.reshape(-1).contiguous()
-        # zeros behind the last column, as the left operand needs them
-        self._zero_tail = K % 16 == 0
+        # (zeros behind the last column, as the left operand needs them?)
+        self._set(shape, rows, scale, K % 16 == 0)
+
+    def _set(self, shape, rows, scale, zero_tail):
+        self._shape, self._rows, self.scale = shape, rows, scale
+        self._flat_scale = scale.reshape(-1).contiguous() \
+            if scale.dim() != 1 or not scale.is_contiguous() else scale
+        self._zero_tail = zero_tail
+        self.pitch = int(rows.stride(0)) if rows.shape[0] > 1 else \
+            (int(shape[-1]) + 15) // 16 * 16
+
+    @classmethod
+    def _of(cls, shape, rows, scale):
+        """What quantize_rows has just written."""
+        q = cls.__new__(cls)
+        q._set(shape, rows, scale.reshape(shape[:-1]), True)
+        return q
 
     @staticmethod
     def _usable(rows):
@@ -1184,12 +1228,6 @@ class QuantizedRows(object):
                 pitch >= (K + 15) // 16 * 16 and
                 rows.data_ptr() % 16 == 0 and
                 end <= rows.untyped_storage().nbytes())
-
-    @staticmethod
-    def _empty(n, K, device):
-        """int8 [n, K] at a pitch of whole 128 bytes, a view of its storage."""
-        return torch.empty(n, (K + 127) // 128 * 128, dtype=torch.int8,
-                           device=device)[:, :K]
 
     @classmethod
     def _padded(cls, rows):
@@ -1212,21 +1250,16 @@ class QuantizedRows(object):
     def device(self):
         return self._rows.device
 
-    @property
-    def pitch(self):
-        return int(self._rows.stride(0)) if self._rows.shape[0] > 1 else \
-            (int(self._shape[-1]) + 15) // 16 * 16
-
     def dequantize(self, dtype=torch.float32):
         """values * scale as a dense tensor."""
         code = row_dtype(dtype, 'dequantize: dtype')
         out = torch.empty(self._shape, dtype=dtype, device=self.device)
         n, K = self._rows.shape
         if n:
-            with torch.cuda.device(self.device):
+            with _capi.on_device(self.device) as stream:
                 _capi.call('zshmc_dequantize_rows', self._rows.data_ptr(),
                            self.pitch, self._flat_scale.data_ptr(), n, K,
-                           out.data_ptr(), K, code, _capi.current_stream())
+                           out.data_ptr(), K, code, stream)
         return out
 
 
@@ -1245,17 +1278,15 @@ def quantize_rows(x):
     require_device(x)
     x2, ldx = _rows_2d(x)
     n, K = x2.shape
-    rows = QuantizedRows._empty(n, K, x.device)
+    pitch = (K + 127) // 128 * 128
+    rows = torch.empty(n, pitch, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=_F32, device=x.device)
     if n:
-        with torch.cuda.device(x.device):
+        with _capi.on_device(x.device) as stream:
             _capi.call('zshmc_quantize_rows', x2.data_ptr(), n, K, ldx, code,
-                       rows.data_ptr(), (K + 127) // 128 * 128,
-                       scale.data_ptr(), _capi.current_stream())
-    q = QuantizedRows.__new__(QuantizedRows)
-    q._shape, q._rows, q._zero_tail = x.shape, rows, True
-    q._flat_scale, q.scale = scale, scale.reshape(x.shape[:-1])
-    return q
+                       rows.data_ptr(), pitch, scale.data_ptr(), stream)
+    return QuantizedRows._of(x.shape, rows if pitch == K else rows[:, :K],
+                             scale)
 
 
 def quantized_linear(w, X, bias=None, dtype=None):
@@ -1264,15 +1295,18 @@ def quantized_linear(w, X, bias=None, dtype=None):
     to 8 bits per row here -- or a `QuantizedRows`.  The integer sum is exact;
     out[..., v] = (scale_x scale_w[v]) * sum + bias[v] in float32, rounded once to
     `dtype` (X's own, float32 for a QuantizedRows).  K <= 131072.  No gradient."""
-    if not isinstance(w, QuantizedRows) or len(w.shape) != 2:
+    if not isinstance(w, QuantizedRows) or len(w._shape) != 2:
         raise TypeError("quantized_linear: w must be QuantizedRows [V, K]")
     X = _symbolic.force(X.tensor if hasattr(X, 'tensor') else X)
     if not isinstance(X, (torch.Tensor, QuantizedRows)):
         raise TypeError("quantized_linear: X must be a tensor or QuantizedRows")
+    if isinstance(X, torch.Tensor):
+        row_dtype(X.dtype, 'quantized_linear: X')
+        require_device(X)
     if dtype is None:
         dtype = X.dtype if isinstance(X, torch.Tensor) else _F32
     code = row_dtype(dtype, 'quantized_linear: dtype')
-    V, K = w.shape
+    V, K = w._shape
     if len(X.shape) < 1 or X.shape[-1] != K or V == 0:
         raise ValueError("quantized_linear: w [V, K] and X [..., K] expected, "
                          "got {} and {}".format(tuple(w.shape),
@@ -1286,23 +1320,31 @@ def quantized_linear(w, X, bias=None, dtype=None):
             raise ValueError("quantized_linear: bias must be a float tensor "
                              "[{}]".format(V))
         require_device(bias)
-        bias = bias.detach().to(_F32).contiguous()
-    if isinstance(X, torch.Tensor):
-        require_device(X)
-    if any(t is not None and t.device != w.device for t in (X, bias)):
+        bias = _float_row(bias)
+    if X.device != w.device or (bias is not None and bias.device != w.device):
         raise ValueError("quantized_linear: all tensors must be on one device")
-    x = quantize_rows(X) if isinstance(X, torch.Tensor) else X
-    rows, pitch = x._rows, x.pitch
-    if not x._zero_tail:
+    out = torch.empty(X.shape[:-1] + (V,), dtype=dtype, device=w.device)
+    if not out.numel():
+        return out
+    if isinstance(X, torch.Tensor):
+        x2, ldx = _rows_2d(X)
+        n = x2.shape[0]
+        size = n * ((K + 127) // 128 * 128 + 4)
+        with _capi.on_device(w.device) as stream:
+            ws = torch.empty(size, dtype=torch.uint8, device=w.device)
+            _capi.call('zshmc_quantized_linear', x2.data_ptr(), ldx,
+                       _ROW_DTYPES[X.dtype], w._rows.data_ptr(), w.pitch,
+                       w._flat_scale.data_ptr(), _capi.ptr(bias), n, K, V,
+                       out.data_ptr(), V, code, ws.data_ptr(), size, stream)
+        return out
+    rows, pitch = X._rows, X.pitch
+    if not X._zero_tail:
         rows = QuantizedRows._padded(rows)
-        pitch = int(rows.stride(0))
-    out = torch.empty(tuple(x.shape[:-1]) + (V,), dtype=dtype,
-                      device=w.device)
-    if rows.shape[0]:
-        with torch.cuda.device(w.device):
-            _capi.call('zshmc_int8_linear', rows.data_ptr(), pitch,
-                       x._flat_scale.data_ptr(), w._rows.data_ptr(), w.pitch,
-                       w._flat_scale.data_ptr(), _capi.ptr(bias),
-                       rows.shape[0], K, V, out.data_ptr(), V, code,
-                       _capi.current_stream())
+        pitch = int(rows.stride(0)) if rows.shape[0] > 1 else \
+            (K + 15) // 16 * 16
+    with _capi.on_device(w.device) as stream:
+        _capi.call('zshmc_int8_linear', rows.data_ptr(), pitch,
+                   X._flat_scale.data_ptr(), w._rows.data_ptr(), w.pitch,
+                   w._flat_scale.data_ptr(), _capi.ptr(bias),
+                   rows.shape[0], K, V, out.data_ptr(), V, code, stream)
     return out

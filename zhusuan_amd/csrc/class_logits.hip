@@ -35,40 +35,55 @@ __device__ __forceinline__ float bf16_value(uint16_t b) {
 }
 
 // ---- operands as the tile loop wants them ------------------------------------
-// rows of `cols` elements -> bfloat16 rows of `pitch` bytes, zero behind the
-// last column; float32 becomes three planes.  Rows whose label is `ignore`
+// rows of `cols` elements -> rows of `pitch` bytes, zero behind the last column:
+// elements as they are, or (SPLIT) float32 as three bfloat16 planes.  Rows whose label is `ignore`
 // become zeros (whatever they hold, NaN included, reaches no product).
-template <bool F32>
-__global__ void pack_rows_kernel(const void* __restrict__ src, int64_t rows, int64_t cols,
+template <typename T, bool SPLIT>
+__global__ void pack_rows_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
                                  int64_t ld, unsigned char* __restrict__ dst, int64_t pitch,
                                  int64_t plane, const int64_t* __restrict__ labels,
                                  int64_t ignore) {
+  constexpr int N = SPLIT ? 8 : 16 / (int)sizeof(T);     // elements per 16 bytes out
   const int64_t groups = pitch / 16;
   const int64_t total = rows * groups;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / groups, c = (i - r * groups) * 8;
+    const int64_t r = i / groups, c = (i - r * groups) * N;
     const bool out = labels && labels[r] == ignore;
-    uint16_t p[3][8];
+    const T* const from = src + r * ld + c;
+    T v[N] = {};
+    if (!out && c + N <= cols) {
+      typedef T any __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+      const any a = *reinterpret_cast<const any*>(from);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = !out && c + e < cols;
-      if constexpr (F32) {
-        const float v = in ? static_cast<const float*>(src)[r * ld + c + e] : 0.f;
-        p[0][e] = bf16_bits(v);
-        const float v1 = v - bf16_value(p[0][e]);
-        p[1][e] = bf16_bits(v1);
-        p[2][e] = bf16_bits(v1 - bf16_value(p[1][e]));
-      } else {
-        p[0][e] = in ? static_cast<const uint16_t*>(src)[r * ld + c + e] : (uint16_t)0;
-      }
+      for (int e = 0; e < N; ++e) v[e] = a[e];
+    } else if (!out) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (c + e < cols) v[e] = from[e];
     }
+    unsigned char* const to = dst + r * pitch + (i - r * groups) * 16;
+    if constexpr (SPLIT) {
+      uint32_t p[3][4];
 #pragma unroll
-    for (int k = 0; k < (F32 ? 3 : 1); ++k) {
-      tu4 v;
+      for (int q = 0; q < 4; ++q) {
+        float a = v[2 * q], b = v[2 * q + 1];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = p[k][2 * q] | (uint32_t)p[k][2 * q + 1] << 16;
-      *reinterpret_cast<tu4*>(dst + k * plane + r * pitch + c * 2) = v;
+        for (int k = 0; k < 3; ++k) {
+          p[k][q] = bf16_pair(a, b);
+          a -= __builtin_bit_cast(float, p[k][q] << 16);
+          b -= __builtin_bit_cast(float, p[k][q] & 0xffff0000u);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<tu4*>(to + k * plane) = tu4{p[k][0], p[k][1], p[k][2], p[k][3]};
+    } else {
+      typedef T whole __attribute__((ext_vector_type(N)));
+      whole w;
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] = v[e];
+      *reinterpret_cast<whole*>(to) = w;
     }
   }
 }
@@ -334,21 +349,29 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 }
 
 // ---- joins ---------------------------------------------------------------------
-// 16 rows x 16 lanes of parts per workgroup
+// ROWS rows x 256 / ROWS lanes of parts per workgroup
+template <int ROWS>
 __global__ __launch_bounds__(256) void join_stats_kernel(
     const cf2* __restrict__ part, int parts, const float* __restrict__ label_logit,
     const int64_t* __restrict__ labels, int64_t n, int64_t n_classes, int has_ignore,
     int64_t ignore, float* __restrict__ log_prob, cf2* __restrict__ stats) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-  const int k = threadIdx.x >> 4;
+  constexpr int kLanes = 256 / ROWS;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x % ROWS;
+  const int k = threadIdx.x / ROWS;
   cf2 t{-__builtin_inff(), 0.f};
   if (row < n)
-    for (int i = k; i < parts; i += 16) t = join(t, part[(int64_t)i * n + row]);
-  __shared__ cf2 s[16][16];
-  s[k][threadIdx.x & 15] = t;
-  __syncthreads();
+    for (int i = k; i < parts; i += kLanes) t = join(t, part[(int64_t)i * n + row]);
+  __shared__ cf2 s[256];
+  s[threadIdx.x] = t;
+#pragma unroll
+  for (int left = kLanes / 2; left > 0; left /= 2) {
+    __syncthreads();
+    if (k < left) {
+      t = join(t, s[threadIdx.x + left * ROWS]);
+      s[threadIdx.x] = t;
+    }
+  }
   if (k || row >= n) return;
-  for (int i = 1; i < 16; ++i) t = join(t, s[i][threadIdx.x & 15]);
   const int64_t y = labels[row];
   float lp = __builtin_nanf("");
   if (has_ignore && y == ignore)
@@ -399,10 +422,21 @@ struct ClassProblem {
   int64_t esize() const { return f32() ? 4 : 2; }
 };
 
-bool direct(const void* p, int64_t ld, int64_t d, const ClassProblem& q) {
-  return !q.f32() && d % 8 == 0 && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
-         ld * 2 <= kMaxPitch;
+// rows that the tile loop can read where they lie
+bool direct(const void* p, int64_t ld, const ClassProblem& q, bool whole) {
+  const int64_t e = q.esize();
+  return (whole || !q.f32()) && q.d * e % 16 == 0 && ld * e % 16 == 0 &&
+         (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * e <= kMaxPitch;
 }
+
+// Up to how many rows float32 operands are multiplied as they are, on
+// v_mfma_f32_32x32x2_f32 (2 N V D flop at 140 TFLOP/s), rather than packed into
+// planes (16 bytes an element of w, then six products at 1250): the two meet near
+// 770 rows.
+constexpr int64_t kWholeRows = 768;
+
+// the logits' tiles: classes x rows of X
+constexpr int kTileClasses[] = {256, 128, 128, 128}, kTileRows[] = {256, 128, 64, 32};
 
 // Where everything lies in the workspace
 struct ClassLayout {
@@ -411,8 +445,9 @@ struct ClassLayout {
   bool pack_x, pack_w;
   int64_t xp, wp;                  // offsets
   int64_t part, label_logit;       // forward
-  int tile;                        // 0: 256 x 256, 1: 128 x 128, 2: 128 classes x 32 rows
-  int64_t tiles_v;
+  int tile;                        // see kTileClasses
+  int64_t tiles_v;                 // parts of the statistics
+  bool whole;                      // float32 operands as they are, no planes
   int64_t piece, pieces;           // gradient: classes per piece
   int64_t resid_pitch, resid_plane;
   int64_t resid, dx_part, bias_part;
@@ -424,10 +459,11 @@ int64_t tiles(int64_t n, int64_t b) { return (n + b - 1) / b; }
 
 ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   ClassLayout l;
-  l.planes = q.f32() ? 3 : 1;
-  l.pitch = round_up(q.d, 64) * 2;
-  l.pack_x = !direct(q.x, q.ldx, q.d, q) || (grad && has_ignore);
-  l.pack_w = !direct(q.w, q.ldw, q.d, q);
+  l.whole = q.f32() && !grad && q.n <= kWholeRows;
+  l.planes = q.f32() && !l.whole ? 3 : 1;
+  l.pitch = round_up(q.d * (l.whole ? 4 : 2), 128);
+  l.pack_x = !direct(q.x, q.ldx, q, l.whole) || (grad && has_ignore);
+  l.pack_w = !direct(q.w, q.ldw, q, l.whole);
   l.x_plane = q.n * l.pitch;
   l.w_plane = q.v * l.pitch;
   const int cus = device_cu_count();
@@ -447,8 +483,10 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   }
   l.pieces = tiles(q.v, l.piece);
   // large tiles where they fill the chip
-  l.tile = q.n <= 32 ? 2 : tiles(l.piece, 256) * tiles(q.n, 256) >= cus ? 0 : 1;
-  l.tiles_v = tiles(q.v, l.tile == 0 ? 256 : 128);
+  l.tile = q.n <= 32                                            ? 3
+           : q.n <= 64                                          ? 2
+           : tiles(l.piece, 256) * tiles(q.n, 256) >= cus ? 0 : 1;
+  l.tiles_v = tiles(q.v, kTileClasses[l.tile]);
   l.part = l.label_logit = l.resid = l.dx_part = l.bias_part = 0;
   if (!grad) {
     l.part = take(l.tiles_v * q.n * 8);
@@ -466,8 +504,7 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     if (s > steps / 4) s = steps / 4;
     l.dx_splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     l.dx_part = take(l.dx_splits * q.n * q.d * 4);
-    const int64_t bn = l.tile == 0 ? 256 : l.tile == 1 ? 128 : 32;
-    l.bias_part = take(tiles(q.n, bn) * q.v * 4);
+    l.bias_part = take(tiles(q.n, kTileRows[l.tile]) * q.v * 4);
   }
   l.total = at;
   return l;
@@ -499,29 +536,35 @@ int launch_tile(const ClassArgs& a, hipStream_t s) {
   return ZSHMC_OK;
 }
 
-template <bool AK, bool BK> using Big = TileCfg<MmaBf16, 2, 2, 4, 4, AK, BK>;
-template <bool AK, bool BK> using Mid = TileCfg<MmaBf16, 2, 2, 2, 2, AK, BK>;
-using Few = TileCfg<MmaBf16, 4, 1, 1, 1, false, false>;
+template <typename M, bool AK, bool BK> using Big = TileCfg<M, 2, 2, 4, 4, AK, BK>;
+template <typename M, bool AK, bool BK> using Mid = TileCfg<M, 2, 2, 2, 2, AK, BK>;
+template <typename M, int WN> using Few = TileCfg<M, 4, 1, 1, WN, false, false>;
 
-template <int EPI, bool F32>
+template <typename M, int EPI, bool F32>
 int launch_logits(const ClassArgs& a, int tile, hipStream_t s) {
   switch (tile) {
-    case 0: return launch_tile<Big<false, false>, EPI, F32>(a, s);
-    case 1: return launch_tile<Mid<false, false>, EPI, F32>(a, s);
-    default: return launch_tile<Few, EPI, F32>(a, s);
+    case 0: return launch_tile<Big<M, false, false>, EPI, F32>(a, s);
+    case 1: return launch_tile<Mid<M, false, false>, EPI, F32>(a, s);
+    case 2: return launch_tile<Few<M, 2>, EPI, F32>(a, s);
+    default: return launch_tile<Few<M, 1>, EPI, F32>(a, s);
   }
 }
 
 int pack_rows(const void* src, int64_t rows, int64_t ld, const ClassProblem& q,
-              unsigned char* dst, int64_t pitch, int64_t plane, const int64_t* labels,
+              const ClassLayout& l, unsigned char* dst, int64_t plane, const int64_t* labels,
               int64_t ignore, hipStream_t s) {
-  const unsigned grid = grid_for(rows * (pitch / 16));
-  if (q.f32())
-    hipLaunchKernelGGL(pack_rows_kernel<true>, dim3(grid), dim3(256), 0, s, src, rows, q.d, ld,
-                       dst, pitch, plane, labels, ignore);
+  const dim3 grid(grid_for(rows * (l.pitch / 16)));
+  const float* f = static_cast<const float*>(src);
+  if (q.f32() && !l.whole)
+    hipLaunchKernelGGL((pack_rows_kernel<float, true>), grid, dim3(256), 0, s, f, rows, q.d, ld,
+                       dst, l.pitch, plane, labels, ignore);
+  else if (q.f32())
+    hipLaunchKernelGGL((pack_rows_kernel<float, false>), grid, dim3(256), 0, s, f, rows, q.d, ld,
+                       dst, l.pitch, plane, labels, ignore);
   else
-    hipLaunchKernelGGL(pack_rows_kernel<false>, dim3(grid), dim3(256), 0, s, src, rows, q.d, ld,
-                       dst, pitch, plane, labels, ignore);
+    hipLaunchKernelGGL((pack_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s,
+                       static_cast<const uint16_t*>(src), rows, q.d, ld, dst, l.pitch, plane,
+                       labels, ignore);
   ZS_LAUNCH_CHECK("pack_rows_kernel launch");
   return ZSHMC_OK;
 }
@@ -532,19 +575,37 @@ int operands(const ClassProblem& q, const ClassLayout& l, unsigned char* ws,
              TileOperand* w) {
   const unsigned char* px = static_cast<const unsigned char*>(q.x);
   const unsigned char* pw = static_cast<const unsigned char*>(q.w);
-  *x = TileOperand{px, q.ldx * 2, 0, q.n, q.d * 2};
-  *w = TileOperand{pw, q.ldw * 2, 0, q.v, q.d * 2};
+  const int64_t e = q.esize();
+  *x = TileOperand{px, q.ldx * e, 0, q.n, q.d * e};
+  *w = TileOperand{pw, q.ldw * e, 0, q.v, q.d * e};
   if (l.pack_x) {
-    const int rc = pack_rows(q.x, q.n, q.ldx, q, ws + l.xp, l.pitch, l.x_plane, drop_labels,
-                             ignore, s);
+    const int rc = pack_rows(q.x, q.n, q.ldx, q, l, ws + l.xp, l.x_plane, drop_labels, ignore,
+                             s);
     if (rc != ZSHMC_OK) return rc;
     *x = TileOperand{ws + l.xp, l.pitch, l.x_plane, q.n, l.pitch};
   }
   if (l.pack_w) {
-    const int rc = pack_rows(q.w, q.v, q.ldw, q, ws + l.wp, l.pitch, l.w_plane, nullptr, 0, s);
+    const int rc = pack_rows(q.w, q.v, q.ldw, q, l, ws + l.wp, l.w_plane, nullptr, 0, s);
     if (rc != ZSHMC_OK) return rc;
     *w = TileOperand{ws + l.wp, l.pitch, l.w_plane, q.v, l.pitch};
   }
+  return ZSHMC_OK;
+}
+
+int join_stats(const ClassProblem& q, const ClassLayout& l, const ClassArgs& a,
+               const int64_t* labels, int has_ignore, int64_t ignore, float* log_prob,
+               float* stats, hipStream_t s) {
+  cf2* st = reinterpret_cast<cf2*>(stats);
+  // a workgroup per row where 16 rows a workgroup leave the chip empty
+  if (q.n <= 16ll * device_cu_count())
+    hipLaunchKernelGGL(join_stats_kernel<2>, dim3((unsigned)tiles(q.n, 2)), dim3(256), 0, s,
+                       a.part, (int)l.tiles_v, a.label_logit, labels, q.n, q.v, has_ignore,
+                       ignore, log_prob, st);
+  else
+    hipLaunchKernelGGL(join_stats_kernel<16>, dim3((unsigned)tiles(q.n, 16)), dim3(256), 0, s,
+                       a.part, (int)l.tiles_v, a.label_logit, labels, q.n, q.v, has_ignore,
+                       ignore, log_prob, st);
+  ZS_LAUNCH_CHECK("join_stats_kernel launch");
   return ZSHMC_OK;
 }
 
@@ -595,25 +656,22 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   ClassArgs a{};
+  a.part = reinterpret_cast<cf2*>(ws + l.part);
+  a.label_logit = reinterpret_cast<float*>(ws + l.label_logit);
   rc = operands(q, l, ws, nullptr, 0, s, &a.b, &a.a);
   if (rc != ZSHMC_OK) return rc;
   a.m = q.v;
   a.n = q.n;
-  a.steps = (int)tiles(q.d, 64);
-  a.terms = q.f32() ? kTerms3 : 1;
+  a.steps = (int)tiles(q.d * (l.whole ? 4 : 2), 128);
+  a.terms = l.planes > 1 ? kTerms3 : 1;
   a.splits = 1;
   a.bias = bias;
   a.labels = labels;
   a.n_classes = q.v;
-  a.part = reinterpret_cast<cf2*>(ws + l.part);
-  a.label_logit = reinterpret_cast<float*>(ws + l.label_logit);
-  rc = launch_logits<kEpiStats, false>(a, l.tile, s);
+  rc = l.whole ? launch_logits<MmaF32, kEpiStats, false>(a, l.tile, s)
+               : launch_logits<MmaBf16, kEpiStats, false>(a, l.tile, s);
   if (rc != ZSHMC_OK) return rc;
-  hipLaunchKernelGGL(join_stats_kernel, dim3((unsigned)tiles(q.n, 16)), dim3(256), 0, s, a.part,
-                     (int)l.tiles_v, a.label_logit, labels, q.n, q.v, has_ignore, ignore_label,
-                     log_prob, reinterpret_cast<cf2*>(stats));
-  ZS_LAUNCH_CHECK("join_stats_kernel launch");
-  return ZSHMC_OK;
+  return join_stats(q, l, a, labels, has_ignore, ignore_label, log_prob, stats, s);
 }
 
 extern "C" int zshmc_class_log_prob_grad(
@@ -676,8 +734,8 @@ extern "C" int zshmc_class_log_prob_grad(
     a.resid_plane = l.resid_plane;
     a.bias_part = grad_bias ? reinterpret_cast<float*>(ws + l.bias_part) : nullptr;
     a.bias_ld = q.v;
-    rc = q.f32() ? launch_logits<kEpiResidual, true>(a, l.tile, s)
-                 : launch_logits<kEpiResidual, false>(a, l.tile, s);
+    rc = q.f32() ? launch_logits<MmaBf16, kEpiResidual, true>(a, l.tile, s)
+                 : launch_logits<MmaBf16, kEpiResidual, false>(a, l.tile, s);
     if (rc != ZSHMC_OK) return rc;
     if (grad_w) {                  // dw = r^T X over the rows of X
       ClassArgs g{};
@@ -691,8 +749,8 @@ extern "C" int zshmc_class_log_prob_grad(
       g.out = static_cast<unsigned char*>(grad_w) + c0 * q.d * q.esize();
       g.out_ld = q.d;
       g.out_bf16 = !q.f32();
-      rc = l.dw_tile == 0 ? launch_tile<Big<true, true>, kEpiStore, false>(g, s)
-                          : launch_tile<Mid<true, true>, kEpiStore, false>(g, s);
+      rc = l.dw_tile == 0 ? launch_tile<Big<MmaBf16, true, true>, kEpiStore, false>(g, s)
+                          : launch_tile<Mid<MmaBf16, true, true>, kEpiStore, false>(g, s);
       if (rc != ZSHMC_OK) return rc;
     }
     if (grad_x) {                  // dX += r w over the piece's classes
@@ -708,8 +766,8 @@ extern "C" int zshmc_class_log_prob_grad(
       g.out_ld = q.d;
       g.out_split = q.n * q.d;
       g.accumulate = c0 > 0;
-      rc = l.dx_tile == 0 ? launch_tile<Big<true, false>, kEpiStore, false>(g, s)
-                          : launch_tile<Mid<true, false>, kEpiStore, false>(g, s);
+      rc = l.dx_tile == 0 ? launch_tile<Big<MmaBf16, true, false>, kEpiStore, false>(g, s)
+                          : launch_tile<Mid<MmaBf16, true, false>, kEpiStore, false>(g, s);
       if (rc != ZSHMC_OK) return rc;
     }
   }
@@ -725,10 +783,9 @@ extern "C" int zshmc_class_log_prob_grad(
     ZS_LAUNCH_CHECK("sum_rows_kernel launch");
   }
   if (grad_bias) {
-    const int64_t bn = l.tile == 0 ? 256 : l.tile == 1 ? 128 : 32;
     hipLaunchKernelGGL(sum_rows_kernel<false>, dim3(grid_for(q.v)), dim3(256), 0, s,
-                       reinterpret_cast<const float*>(ws + l.bias_part), (int)tiles(q.n, bn),
-                       q.v, q.v, grad_bias);
+                       reinterpret_cast<const float*>(ws + l.bias_part),
+                       (int)tiles(q.n, kTileRows[l.tile]), q.v, q.v, grad_bias);
     ZS_LAUNCH_CHECK("sum_rows_kernel launch");
   }
   return ZSHMC_OK;

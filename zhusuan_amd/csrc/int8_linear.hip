@@ -46,104 +46,163 @@ struct RowVec<uint16_t> {
   }
 };
 
-// the 16 bytes from column c on, zero from `cols` on
-template <typename T>
-__device__ __forceinline__ tu4 load_row(const T* row, int64_t c, int64_t cols) {
-  constexpr int N = RowVec<T>::N;
-  if (c + N <= cols) return *reinterpret_cast<const tu4_any*>(row + c);
-  tu4 v{};
+__device__ __forceinline__ float element(const float* row, int c) { return row[c]; }
+__device__ __forceinline__ float element(const uint16_t* row, int c) {
+  return __builtin_bit_cast(float, (uint32_t)row[c] << 16);
+}
+
+// N values -> N / 4 words of rint(f / s), f / s rounded to float32 first.  One
+// fma with the reciprocal and 1.5 * 2^23 rounds to the integer in the low byte; it
+// says which integer unless the quotient falls within 2^-12 of the middle of two
+// (the product's error is below 127 * 3 * 2^-24) or `inv` is NaN: then the division
+// does, for all N (|f| / s <= 127 (1 + 2^-23) unless s is subnormal).
+template <int N>
+__device__ __forceinline__ void quotients(const float (&f)[N], float s, float inv,
+                                          uint32_t (&w)[N / 4]) {
+  constexpr float kMagic = 12582912.f;
+  float y[N];
+  bool near = false;
 #pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (c + e < cols) {
-      if constexpr (N == 4)
-        v[e] = __builtin_bit_cast(uint32_t, row[c + e]);
-      else
-        v[e / 2] |= (uint32_t)row[c + e] << (16 * (e & 1));
+  for (int e = 0; e < N; ++e) {
+    y[e] = __builtin_fmaf(f[e], inv, kMagic);
+    near |= !(fabsf(f[e] * inv - (y[e] - kMagic)) <= 0.5f - 0x1p-12f);
+  }
+  if (near) {
+#pragma unroll 1
+    for (int e = 0; e < N; ++e) {
+      float d = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) d = e == k ? f[k] : d;
+      d = fminf(fmaxf(rintf(d / s), -127.f), 127.f) + kMagic;
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[k] = e == k ? d : y[k];
     }
-  return v;
+  }
+#pragma unroll
+  for (int k = 0; k < N / 4; ++k) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = y[4 * k + e];
+      b[e] = __builtin_bit_cast(uint32_t, v);
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+    w[k] = lo | hi << 16;
+  }
 }
 
-// rint(x / s), x / s rounded to float32 first: a product with the reciprocal
-// says which integer unless it falls within 2^-12 of the middle of two (its error
-// is below 127 * 3 * 2^-24), then the division does.
-__device__ __forceinline__ float quotient(float x, float s, float inv) {
-  const float t = x * inv;
-  float q = rintf(t);
-  if (fabsf(t - q) > 0.5f - 0x1p-12f) q = rintf(x / s);
-  return fminf(fmaxf(q, -127.f), 127.f);
+// One row by TPR threads (thread t).  Thread t's k-th vector is columns c .. c + N - 1,
+// c = (k TPR + t) N; one that reaches past the row's end is read from cols - N
+// instead, so that every load is a whole vector inside the row and needs no mask
+// (a value seen twice changes no maximum).  put(c, words) stores a whole vector's N / 4
+// words, put1(c, byte) one column of the last, up to `width` columns with zeros
+// from `cols` on.  Returns the scale.
+template <typename T, int TPR, typename P, typename P1>
+__device__ __forceinline__ float quantize_row(const T* row, int cols, int width, int t,
+                                              float* part, P&& put, P1&& put1) {
+  constexpr int N = RowVec<T>::N;
+  float mx = 0.f;
+  // a NaN or an infinity turns into a maximum no finite row reaches
+  auto widen = [&](float f) {
+    const float a = fabsf(f);
+    mx = a <= 3.402823466e38f ? fmaxf(mx, a) : __builtin_inff();
+  };
+  auto load = [&](int c) -> tu4 {
+    return *reinterpret_cast<const tu4_any*>(row + (c + N <= cols ? c : cols - N));
+  };
+  auto widen_all = [&](const tu4& v) {
+    float f[N];
+    RowVec<T>::unpack(v, f);
+#pragma unroll
+    for (int e = 0; e < N; ++e) widen(f[e]);
+  };
+  tu4 held[kHeld];
+  const bool tiny = cols < N;              // less than a vector: element by element
+  if (!tiny) {
+    tile_for<kHeld>([&](auto K) {
+      constexpr int k = decltype(K)::value;
+      if (k * TPR * N < cols) held[k] = load((k * TPR + t) * N);
+    });
+    tile_for<kHeld>([&](auto K) {
+      constexpr int k = decltype(K)::value;
+      if (k * TPR * N < cols) widen_all(held[k]);
+    });
+#pragma unroll 1
+    for (int c = (kHeld * TPR + t) * N; c < cols; c += TPR * N) widen_all(load(c));
+  } else {
+    for (int c = 0; c < cols; ++c) widen(element(row, c));
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  if constexpr (TPR == 256) {
+    __syncthreads();
+    if ((t & 63) == 0) part[t >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  }
+  const bool bad = mx == __builtin_inff();
+  float s = mx / 127.f;
+  if (s == 0.f) s = 1.f;
+  // (a subnormal scale has no float32 reciprocal: every quotient is divided)
+  const float inv = s >= 0x1p-120f ? 1.f / s : __builtin_nanf("");
+  auto store = [&](const tu4& v, int c) {
+    float f[N];
+    uint32_t w[N / 4];
+    RowVec<T>::unpack(v, f);
+    quotients<N>(f, s, inv, w);
+    if (bad || c >= cols)
+#pragma unroll
+      for (int e = 0; e < N / 4; ++e) w[e] = 0;
+    if (c + N <= cols || c >= cols) {
+      if (c < width) put(c, w);
+      return;
+    }
+    // the row's end: the vector starts at cols - N
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int col = cols - N + e;
+      if (col >= c) put1(col, (uint8_t)(w[e / 4] >> (8 * (e & 3))));
+      if (col + N < c + N && col + N >= cols) put1(col + N, (uint8_t)0);
+    }
+  };
+  if (!tiny) {
+    tile_for<kHeld>([&](auto K) {
+      constexpr int k = decltype(K)::value;
+      if (k * TPR * N < width) store(k * TPR * N < cols ? held[k] : tu4{}, (k * TPR + t) * N);
+    });
+#pragma unroll 1
+    for (int c = (kHeld * TPR + t) * N; c < width; c += TPR * N)
+      store(c < cols ? load(c) : tu4{}, c);
+  } else {
+    for (int c = t; c < width; c += TPR) {
+      float q = 0.f;
+      if (c < cols && !bad) q = fminf(fmaxf(rintf(element(row, c) / s), -127.f), 127.f);
+      put1(c, (uint8_t)(int8_t)(int)q);
+    }
+  }
+  return bad ? __builtin_nanf("") : s;
 }
 
+// (one row per TPR threads and no loop over rows: hoisted out of one, the columns'
+// masks and offsets take 240 registers)
 template <typename T, int TPR>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(
-    const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int8_t* __restrict__ q,
-    int64_t pitch, float* __restrict__ scale) {
-  constexpr int N = RowVec<T>::N, RPB = 256 / TPR;
+    const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int8_t* __restrict__ q,
+    int pitch, float* __restrict__ scale) {
   const int t = threadIdx.x % TPR;
   __shared__ float part[4];
-  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; r < rows;
-       r += (int64_t)gridDim.x * RPB) {
-    const T* row = x + r * ldx;
-    tu4 held[kHeld];
-    float mx = 0.f;
-    auto widen = [&](const tu4& v) {
-      float f[N];
-      RowVec<T>::unpack(v, f);
-      // a NaN or an infinity turns into a maximum no finite row reaches
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float a = fabsf(f[e]);
-        mx = a <= 3.402823466e38f ? fmaxf(mx, a) : __builtin_inff();
-      }
-    };
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      held[k] = tu4{};
-      const int64_t c = (int64_t)(k * TPR + t) * N;
-      if (c < cols) held[k] = load_row(row, c, cols);
-    }
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) widen(held[k]);
-    for (int64_t c = (int64_t)(kHeld * TPR + t) * N; c < cols; c += TPR * N)
-      widen(load_row(row, c, cols));
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-    if constexpr (TPR == 256) {
-      __syncthreads();
-      if ((t & 63) == 0) part[t >> 6] = mx;
-      __syncthreads();
-      mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    }
-    const bool bad = mx == __builtin_inff();
-    float s = mx / 127.f;
-    if (s == 0.f) s = 1.f;
-    if (t == 0) scale[r] = bad ? __builtin_nanf("") : s;
-    // (a subnormal scale has no float32 reciprocal: every quotient is divided)
-    const float inv = s >= 0x1p-120f ? 1.f / s : __builtin_nanf("");
-    auto store = [&](const tu4& v, int64_t c) {
-      float f[N];
-      RowVec<T>::unpack(v, f);
-      uint32_t w[N / 4];
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        float n = inv == inv ? quotient(f[e], s, inv)
-                             : fminf(fmaxf(rintf(f[e] / s), -127.f), 127.f);
-        n = bad ? 0.f : n;
-        const uint32_t b = (uint32_t)(int)n & 0xffu;
-        w[e / 4] = e % 4 == 0 ? b : w[e / 4] | b << (8 * (e % 4));
-      }
-      if constexpr (N == 4)
-        *reinterpret_cast<uint32_t*>(q + r * pitch + c) = w[0];
-      else
-        *reinterpret_cast<tu2*>(q + r * pitch + c) = tu2{w[0], w[1]};
-    };
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int64_t c = (int64_t)(k * TPR + t) * N;
-      if (c < pitch) store(held[k], c);
-    }
-    for (int64_t c = (int64_t)(kHeld * TPR + t) * N; c < pitch; c += TPR * N)
-      store(c < cols ? load_row(row, c, cols) : tu4{}, c);
-  }
+  const int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (r >= rows) return;                   // (whole waves; TPR = 256: never)
+  int8_t* const out = q + r * pitch;
+  const float s = quantize_row<T, TPR>(x + r * ldx, cols, pitch, t, part,
+                                       [&](int c, const uint32_t* w) {
+    if constexpr (RowVec<T>::N == 4)
+      *reinterpret_cast<uint32_t*>(out + c) = w[0];
+    else
+      *reinterpret_cast<tu2*>(out + c) = tu2{w[0], w[1]};
+  }, [&](int c, uint8_t b) { out[c] = (int8_t)b; });
+  if (t == 0) scale[r] = s;
 }
 
 // 8 values per thread
@@ -280,8 +339,8 @@ int launch_int8(const Int8Args& a, hipStream_t s) {
 }
 
 using BigI8 = TileCfg<MmaI8, 2, 2, 4, 4, false, false>;
-using MidI8 = TileCfg<MmaI8, 2, 2, 2, 2, false, false>;
 using FewI8 = TileCfg<MmaI8, 4, 1, 1, 1, false, false>;
+using MidI8 = TileCfg<MmaI8, 2, 2, 2, 2, false, false>;
 
 unsigned rows_grid(int64_t rows) {
   const int64_t b = (rows + 3) / 4;
@@ -293,41 +352,89 @@ unsigned rows_grid(int64_t rows) {
 
 using namespace zshmc;
 
+namespace {
+int launch_quantize(const void* x, int64_t n_rows, int64_t n_cols, int64_t ldx, int dtype,
+                    int8_t* values, int64_t pitch, float* scale, hipStream_t s) {
+  // a wave per row where that is eight waves a CU or more
+  const bool wave = n_rows >= 8ll * device_cu_count();
+  const unsigned grid = (unsigned)(wave ? (n_rows + 3) / 4 : n_rows);
+  if (dtype == ZSHMC_DTYPE_F32) {
+    const float* f = static_cast<const float*>(x);
+    if (wave)
+      hipLaunchKernelGGL((quantize_rows_kernel<float, 64>), dim3(grid), dim3(256), 0, s, f, n_rows,
+                         (int)n_cols, ldx, values, (int)pitch, scale);
+    else
+      hipLaunchKernelGGL((quantize_rows_kernel<float, 256>), dim3(grid), dim3(256), 0, s, f,
+                         n_rows, (int)n_cols, ldx, values, (int)pitch, scale);
+  } else {
+    const uint16_t* f = static_cast<const uint16_t*>(x);
+    if (wave)
+      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, 64>), dim3(grid), dim3(256), 0, s, f,
+                         n_rows, (int)n_cols, ldx, values, (int)pitch, scale);
+    else
+      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, 256>), dim3(grid), dim3(256), 0, s, f,
+                         n_rows, (int)n_cols, ldx, values, (int)pitch, scale);
+  }
+  ZS_LAUNCH_CHECK("quantize_rows_kernel launch");
+  return ZSHMC_OK;
+}
+
+int check_linear(int64_t n_rows, int64_t n_features, int64_t n_channels, const int8_t* w,
+                 int64_t w_pitch, const void* out, int64_t ldo, int dtype, const char* who) {
+  ZS_REQUIRE(dtype == ZSHMC_DTYPE_F32 || dtype == ZSHMC_DTYPE_BF16,
+             "%s: dtype must be ZSHMC_DTYPE_F32 or _BF16, got %d", who, dtype);
+  ZS_REQUIRE(n_rows >= 0 && n_channels > 0 && n_features > 0 && n_features <= 131072,
+             "%s: n_rows >= 0, n_channels > 0, 1 .. 131072 features (an int32 holds the sum), "
+             "got %lld", who, (long long)n_features);
+  ZS_REQUIRE(w_pitch >= (n_features + 15) / 16 * 16 && w_pitch % 16 == 0 &&
+                 w_pitch <= (4ll << 20) && (reinterpret_cast<uintptr_t>(w) & 15) == 0 &&
+                 ldo >= n_channels,
+             "%s: rows of whole 16 bytes, 16-byte aligned; ldo >= n_channels", who);
+  ZS_REQUIRE(n_rows < (1ll << 31) && n_channels < (1ll << 31),
+             "%s: at most 2^31 - 1 rows and channels", who);
+  return ZSHMC_OK;
+}
+
+// the product of 8-bit rows
+int product(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* w,
+            int64_t w_pitch, const float* w_scale, const float* bias, int64_t n_rows,
+            int64_t n_features, int64_t n_channels, void* out, int64_t ldo, bool bf16,
+            hipStream_t s) {
+  const int64_t bytes = (n_features + 15) / 16 * 16;
+  Int8Args a{};
+  a.a = TileOperand{reinterpret_cast<const unsigned char*>(w), w_pitch, 0, n_channels, bytes};
+  a.b = TileOperand{reinterpret_cast<const unsigned char*>(x), x_pitch, 0, n_rows, bytes};
+  a.m = n_channels;
+  a.n = n_rows;
+  a.steps = (int)((bytes + 127) / 128);
+  a.sx = x_scale;
+  a.sw = w_scale;
+  a.bias = bias;
+  a.out = out;
+  a.ldo = ldo;
+  if (n_rows <= 32)
+    return bf16 ? launch_int8<FewI8, true>(a, s) : launch_int8<FewI8, false>(a, s);
+  const int64_t big = ((n_rows + 255) / 256) * ((n_channels + 255) / 256);
+  if (big >= device_cu_count())
+    return bf16 ? launch_int8<BigI8, true>(a, s) : launch_int8<BigI8, false>(a, s);
+  return bf16 ? launch_int8<MidI8, true>(a, s) : launch_int8<MidI8, false>(a, s);
+}
+}  // namespace
+
 extern "C" int zshmc_quantize_rows(const void* x, int64_t n_rows, int64_t n_cols, int64_t ldx,
                                    int dtype, int8_t* values, int64_t pitch, float* scale,
                                    void* stream) {
   ZS_REQUIRE(dtype == ZSHMC_DTYPE_F32 || dtype == ZSHMC_DTYPE_BF16,
              "zshmc_quantize_rows: dtype must be ZSHMC_DTYPE_F32 or _BF16, got %d", dtype);
-  ZS_REQUIRE(n_rows >= 0 && n_cols > 0 && ldx >= n_cols,
-             "zshmc_quantize_rows: n_rows >= 0, n_cols > 0, ldx >= n_cols");
+  ZS_REQUIRE(n_rows >= 0 && n_rows < (1ll << 31) && n_cols > 0 && n_cols < (1ll << 30) &&
+                 pitch < (1ll << 30) && ldx >= n_cols,
+             "zshmc_quantize_rows: 0 .. 2^31 - 1 rows, 1 .. 2^30 - 1 columns, ldx >= n_cols");
   ZS_REQUIRE(pitch >= n_cols && pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(values) & 15) == 0,
              "zshmc_quantize_rows: values 16-byte aligned with a pitch of whole 16 bytes");
   if (n_rows == 0) return ZSHMC_OK;
   ZS_REQUIRE(x && values && scale, "zshmc_quantize_rows: null pointer");
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  // a wave per row where that is eight waves a CU or more
-  const bool wave = n_rows >= 8ll * device_cu_count();
-  const unsigned grid = wave ? rows_grid(n_rows)
-                             : (unsigned)n_rows;
-  if (dtype == ZSHMC_DTYPE_F32) {
-    const float* f = static_cast<const float*>(x);
-    if (wave)
-      hipLaunchKernelGGL((quantize_rows_kernel<float, 64>), dim3(grid), dim3(256), 0, s, f, n_rows,
-                         n_cols, ldx, values, pitch, scale);
-    else
-      hipLaunchKernelGGL((quantize_rows_kernel<float, 256>), dim3(grid), dim3(256), 0, s, f,
-                         n_rows, n_cols, ldx, values, pitch, scale);
-  } else {
-    const uint16_t* f = static_cast<const uint16_t*>(x);
-    if (wave)
-      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, 64>), dim3(grid), dim3(256), 0, s, f,
-                         n_rows, n_cols, ldx, values, pitch, scale);
-    else
-      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, 256>), dim3(grid), dim3(256), 0, s, f,
-                         n_rows, n_cols, ldx, values, pitch, scale);
-  }
-  ZS_LAUNCH_CHECK("quantize_rows_kernel launch");
-  return ZSHMC_OK;
+  return launch_quantize(x, n_rows, n_cols, ldx, dtype, values, pitch, scale,
+                         reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int zshmc_dequantize_rows(const int8_t* values, int64_t pitch, const float* scale,
@@ -357,38 +464,42 @@ extern "C" int zshmc_int8_linear(const int8_t* x, int64_t x_pitch, const float* 
                                  const float* bias, int64_t n_rows, int64_t n_features,
                                  int64_t n_channels, void* out, int64_t ldo, int dtype,
                                  void* stream) {
-  ZS_REQUIRE(dtype == ZSHMC_DTYPE_F32 || dtype == ZSHMC_DTYPE_BF16,
-             "zshmc_int8_linear: dtype must be ZSHMC_DTYPE_F32 or _BF16, got %d", dtype);
-  ZS_REQUIRE(n_rows >= 0 && n_channels > 0 && n_features > 0 && n_features <= 131072,
-             "zshmc_int8_linear: n_rows >= 0, n_channels > 0, 1 .. 131072 features (an int32 "
-             "holds the sum), got %lld", (long long)n_features);
-  const int64_t bytes = (n_features + 15) / 16 * 16;
-  ZS_REQUIRE(x_pitch >= bytes && w_pitch >= bytes && x_pitch % 16 == 0 && w_pitch % 16 == 0 &&
-                 x_pitch <= (4ll << 20) && w_pitch <= (4ll << 20) &&
-                 (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
-                 (reinterpret_cast<uintptr_t>(w) & 15) == 0 && ldo >= n_channels,
-             "zshmc_int8_linear: rows of whole 16 bytes, 16-byte aligned; ldo >= n_channels");
-  ZS_REQUIRE(n_rows < (1ll << 31) && ldo < (1ll << 22),
-             "zshmc_int8_linear: at most 2^31 - 1 rows and 2^22 - 1 channels");
+  const int rc = check_linear(n_rows, n_features, n_channels, w, w_pitch, out, ldo, dtype,
+                              "zshmc_int8_linear");
+  if (rc != ZSHMC_OK) return rc;
+  ZS_REQUIRE(x_pitch >= (n_features + 15) / 16 * 16 && x_pitch % 16 == 0 &&
+                 x_pitch <= (4ll << 20) && (reinterpret_cast<uintptr_t>(x) & 15) == 0,
+             "zshmc_int8_linear: rows of whole 16 bytes, 16-byte aligned");
   if (n_rows == 0) return ZSHMC_OK;
   ZS_REQUIRE(x && w && x_scale && w_scale && out, "zshmc_int8_linear: null pointer");
-  Int8Args a{};
-  a.a = TileOperand{reinterpret_cast<const unsigned char*>(w), w_pitch, 0, n_channels, bytes};
-  a.b = TileOperand{reinterpret_cast<const unsigned char*>(x), x_pitch, 0, n_rows, bytes};
-  a.m = n_channels;
-  a.n = n_rows;
-  a.steps = (int)((bytes + 127) / 128);
-  a.sx = x_scale;
-  a.sw = w_scale;
-  a.bias = bias;
-  a.out = out;
-  a.ldo = ldo;
+  return product(x, x_pitch, x_scale, w, w_pitch, w_scale, bias, n_rows, n_features, n_channels,
+                 out, ldo, dtype == ZSHMC_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int zshmc_quantized_linear(const void* x, int64_t ldx, int x_dtype, const int8_t* w,
+                                      int64_t w_pitch, const float* w_scale, const float* bias,
+                                      int64_t n_rows, int64_t n_features, int64_t n_channels,
+                                      void* out, int64_t ldo, int dtype, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  const int rc = check_linear(n_rows, n_features, n_channels, w, w_pitch, out, ldo, dtype,
+                              "zshmc_quantized_linear");
+  if (rc != ZSHMC_OK) return rc;
+  ZS_REQUIRE(x_dtype == ZSHMC_DTYPE_F32 || x_dtype == ZSHMC_DTYPE_BF16,
+             "zshmc_quantized_linear: x_dtype must be ZSHMC_DTYPE_F32 or _BF16, got %d", x_dtype);
+  ZS_REQUIRE(ldx >= n_features, "zshmc_quantized_linear: rows overlap (ldx < n_features)");
+  if (n_rows == 0) return ZSHMC_OK;
+  ZS_REQUIRE(x && w && w_scale && out, "zshmc_quantized_linear: null pointer");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool bf16 = dtype == ZSHMC_DTYPE_BF16;
-  const int64_t big = ((n_rows + 255) / 256) * ((n_channels + 255) / 256);
-  if (n_rows <= 32)
-    return bf16 ? launch_int8<FewI8, true>(a, s) : launch_int8<FewI8, false>(a, s);
-  if (big >= device_cu_count())
-    return bf16 ? launch_int8<BigI8, true>(a, s) : launch_int8<BigI8, false>(a, s);
-  return bf16 ? launch_int8<MidI8, true>(a, s) : launch_int8<MidI8, false>(a, s);
+  const int64_t pitch = (n_features + 127) / 128 * 128;
+  ZS_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
+                 workspace_bytes >= n_rows * (pitch + 4),
+             "zshmc_quantized_linear: n_rows * (n_features rounded up to 128, + 4) bytes of "
+             "16-byte aligned workspace needed, got %lld", (long long)workspace_bytes);
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(q + n_rows * pitch);
+  const int rq = launch_quantize(x, n_rows, n_features, ldx, x_dtype, q, pitch, scale, s);
+  if (rq != ZSHMC_OK) return rq;
+  return product(q, pitch, scale, w, w_pitch, w_scale, bias, n_rows, n_features, n_channels, out,
+                 ldo, bf16, s);
 }

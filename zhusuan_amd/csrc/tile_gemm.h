@@ -81,6 +81,18 @@ struct MmaBf16 {
         __builtin_bit_cast(tb8, a), __builtin_bit_cast(tb8, b), c, 0, 0, 0);
   }
 };
+// float32 as it is: a lane's four elements of a chunk one MFMA each (k is a dummy
+// index; both operands hold the same four)
+struct MmaF32 {
+  typedef tf16 Acc;
+  static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, Acc c) {
+    const tf4 x = __builtin_bit_cast(tf4, a), y = __builtin_bit_cast(tf4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  }
+};
 struct MmaI8 {
   typedef ti16 Acc;
   static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {

@@ -13,12 +13,15 @@ def class_log_prob(w, X, labels, bias=None, ignore=None, g=None):
     inputs' device.
 
     The bounds.  A logit is a sum of D products in float32, in any order: off by
-    at most D u sum|x w| (u = 2^-24); three bfloat16 planes per factor make it
-    6 D products and drop terms of 2^-24 sum|x w|.  log-sum-exp moves by no
+    at most D u sum|x w| (u = 2^-24).  float32 factors in two float16 parts make
+    it 3 D products, hold a factor to 2^-23 (2 u) and drop the product of the
+    lower parts, 2^-22 (4 u): (3 D + 8) u in all, less than (6 D + 1) u from D = 3
+    on; the same for the products with r.  (What lies below 2^-38 of an operand's
+    largest value is lost as well.)  log-sum-exp moves by no
     more than its arguments; its exponentials are 2^-23 (1 + |l - M|) off -- at
     the 2^-22 |l - M| <= 2^-22 * 64 where they still count -- and summed over
     at most 300 terms one after the other.  r is rounded to the operands' type
-    (float32: three planes, 2^-24) and g p moves by its logit, M and S.  A
+    and g p moves by its logit, M and S.  A
     product over k terms adds k u times the sum of magnitudes; the result is
     rounded once to its type."""
     wd, xd = w.detach().double(), X.detach().double()

@@ -34,7 +34,8 @@ def check(w, X, y, b, g, ignore=None):
 @pytest.mark.parametrize('N,D,V', [
     (1, 1, 1), (1, 64, 128), (2, 7, 3), (5, 8, 257), (31, 64, 300),
     (32, 130, 129), (33, 128, 500), (64, 100, 777), (65, 200, 1000), (129, 72, 4099),
-    (100, 128, 12419), (300, 256, 40000), (1021, 784, 1237)])
+    (81, 64, 300), (100, 128, 12419), (260, 60, 1000), (300, 256, 40000),
+    (1021, 784, 1237)])
 def test_log_prob_and_gradients(N, D, V, dtype):
     for bias, ignore in ((False, None), (True, IGNORE)):
         w, X, y, b, g = problem(N, D, V, dtype, N + D + V, bias, ignore)
@@ -63,6 +64,31 @@ def test_ignored_rows_may_hold_anything(dtype):
         assert torch.equal(a, c)
     assert bool((lp[y == IGNORE] == 0).all())
     assert bool((grads[1][y == IGNORE] == 0).all())
+
+
+@pytest.mark.parametrize('N', [70, 300])
+@pytest.mark.parametrize('dtype', BOTH)
+def test_ignored_rows_set_no_scale(dtype, N):
+    """Finite, but 1e30 times the others."""
+    w, X, y, b, g = problem(N, 96, 333, dtype, 5, True, IGNORE)
+    X = X.clone()
+    X[y == IGNORE] = 1e30
+    g[y == IGNORE] = 1e30
+    check(w, X, y, b, g, IGNORE)
+
+
+def test_rows_of_different_sizes():
+    """float32 rows from 2^-12 to 2^12 times the others, in X, w and g: every
+    result within its own row's bound (float16 planes hold 2^-38 of an
+    operand's largest value)."""
+    for N in (60, 300):
+        w, X, y, b, g = problem(N, 96, 700, torch.float32, 55)
+        k = torch.arange(N, device='cuda') % 5 - 2
+        X = X * 2.0 ** (4 * k[:, None].clamp(max=0)).float()
+        g = g * 2.0 ** (6 * k).float()
+        w = w * 2.0 ** (4.0 * (torch.arange(700, device='cuda') % 4 - 3)
+                        )[:, None].float()
+        check(w, X, y, b, g)
 
 
 @pytest.mark.parametrize('dtype', BOTH)

@@ -11,11 +11,16 @@
 // Forward: one tile product (tile_gemm.h) whose epilogue leaves, per 256
 // classes, each row's maximum and sum (8 bytes per row instead of 512 of
 // logits), and one pass that joins them.  Gradient: per piece of classes, the
-// logits again, turned into r in the epilogue (bfloat16, or three bfloat16
-// planes for float32 operands), then the two products over that piece; dX is
+// logits again, turned into r in the epilogue (bfloat16, or for float32 operands
+// float32 or two float16 planes), then the two products over that piece; dX is
 // accumulated in float32 over the pieces.  8 N V D flop for both directions,
 // six of them unavoidable.  M and S are float32; r is rounded to the operands'
 // precision because it is an operand of the matrix cores.
+//
+// float32 operands go one of two ways.  Few rows: as they are, on
+// v_mfma_f32_32x32x2_f32.  More: as two float16 planes each (tile_gemm.h), of x /
+// 2^e with one e per operand (w, X, g), found by a pass over them; three products
+// on the 16-bit matrix cores are three times as fast.
 #include "tile_gemm.h"
 
 namespace zshmc {
@@ -34,50 +39,143 @@ __device__ __forceinline__ float bf16_value(uint16_t b) {
   return __builtin_bit_cast(float, (uint32_t)b << 16);
 }
 
+// what float16 leaves of x (nothing of an infinity)
+__device__ __forceinline__ float f16_rest(float x) {
+  const float h = (float)(_Float16)x;
+  return fabsf(h) == __builtin_inff() ? 0.f : x - h;
+}
+
 // ---- operands as the tile loop wants them ------------------------------------
-// rows of `cols` elements -> rows of `pitch` bytes, zero behind the last column:
-// elements as they are, or (SPLIT) float32 as three bfloat16 planes.  Rows whose label is `ignore`
-// become zeros (whatever they hold, NaN included, reaches no product).
-template <typename T, bool SPLIT>
-__global__ void pack_rows_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
-                                 int64_t ld, unsigned char* __restrict__ dst, int64_t pitch,
-                                 int64_t plane, const int64_t* __restrict__ labels,
-                                 int64_t ignore) {
-  constexpr int N = SPLIT ? 8 : 16 / (int)sizeof(T);     // elements per 16 bytes out
-  const int64_t groups = pitch / 16;
-  const int64_t total = rows * groups;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / groups, c = (i - r * groups) * N;
-    const bool out = labels && labels[r] == ignore;
-    const T* const from = src + r * ld + c;
-    T v[N] = {};
-    if (!out && c + N <= cols) {
-      typedef T any __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-      const any a = *reinterpret_cast<const any*>(from);
+// The power of two that brings a magnitude near 2^14: 2^(its exponent - 13), 2^-113
+// and more, so that the reciprocal is a number; 1 for zeros and what is no number.
+__device__ __forceinline__ float near_2_14(float x) {
+  int e = (int)(__builtin_bit_cast(uint32_t, fabsf(x)) >> 23) - 127;
+  if (x == 0.f || e == 128) return 1.f;
+  e = e < -100 ? -100 : e;
+  return __builtin_bit_cast(float, (uint32_t)(e - 13 + 127) << 23);
+}
+
+// Rows to be packed, and the largest finite magnitudes of X, w and g that their
+// scales come from, per workgroup, without the rows (of X and g) that are ignored.
+constexpr int kMaxParts = 1024;
+struct PackJob {
+  const void* src;
+  int64_t rows, cols, ld;
+  unsigned char* dst;
+  const int64_t* labels;           // rows labelled `ignore` become zeros; or NULL
+  const float* row_g;              // rows are scaled like g's: or NULL
+  int part, part_g;                // whose maximum
+  int writes;                      // the first workgroup writes scale[part] ( + [part_g])
+};
+struct PackArgs {
+  PackJob job[3];
+  int64_t pitch, ignore;
+  const float* part;               // [3][kMaxParts]
+  float* scale;                    // [3]
+};
+
+__global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* __restrict__ g,
+                                                       float* __restrict__ part) {
+  const int k = blockIdx.y;
+  // X, w, g: the third has one column
+  const PackJob& j = a.job[k == 1 ? 1 : 0];
+  const float* src = k == 2 ? g : static_cast<const float*>(j.src);
+  const int64_t rows = k == 2 && !g ? 0 : j.rows, cols = k == 2 ? 1 : j.cols;
+  const int64_t ld = k == 2 ? 1 : j.ld, groups = (cols + 3) / 4, total = rows * groups;
+  float mx = 0.f;
+  auto widen = [&](float v) {
+    v = fabsf(v);
+    mx = v <= 3.402823466e38f ? fmaxf(mx, v) : mx;
+  };
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = (i - r * groups) * 4;
+    if (j.labels && j.labels[r] == a.ignore) continue;
+    const float* from = src + r * ld + c;
+    if (c + 4 <= cols) {
+      typedef float any __attribute__((ext_vector_type(4), aligned(4)));
+      const any v = *reinterpret_cast<const any*>(from);
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = a[e];
+      for (int e = 0; e < 4; ++e) widen(v[e]);
+    } else {
+      for (int e = 0; e < cols - c; ++e) widen(from[e]);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  __shared__ float s[4];
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    part[k * kMaxParts + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+
+// blockIdx.y's rows of `cols` elements -> rows of `pitch` bytes, zero behind the
+// last column: elements as they are, or (SPLIT) float32 as two float16 planes of x /
+// scale.  Rows whose label is `ignore` become zeros (whatever they hold, NaN
+// included, reaches no product).
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
+  constexpr int N = SPLIT ? 8 : 16 / (int)sizeof(T);     // elements per 16 bytes out
+  const PackJob& j = a.job[blockIdx.y];
+  const int64_t groups = a.pitch / 16, total = j.rows * groups, plane = j.rows * a.pitch;
+  if ((int64_t)blockIdx.x * 256 >= total) return;
+  float inv = 1.f, inv_g = 1.f;
+  if (SPLIT) {
+    __shared__ float s[2][4];
+    float mx = 0.f, mg = 0.f;
+    for (int i = threadIdx.x; i < kMaxParts; i += 256) {
+      mx = fmaxf(mx, a.part[j.part * kMaxParts + i]);
+      mg = fmaxf(mg, a.part[j.part_g * kMaxParts + i]);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+      mg = fmaxf(mg, __shfl_xor(mg, off, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+      s[0][threadIdx.x >> 6] = mx;
+      s[1][threadIdx.x >> 6] = mg;
+    }
+    __syncthreads();
+    const float scale = near_2_14(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])));
+    const float scale_g = near_2_14(fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    inv = 1.f / scale;
+    inv_g = 1.f / scale_g;
+    if (j.writes && blockIdx.x == 0 && threadIdx.x == 0) {
+      a.scale[j.part] = scale;
+      if (j.part_g != j.part) a.scale[j.part_g] = scale_g;
+    }
+  }
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = (i - r * groups) * N;
+    const bool out = j.labels && j.labels[r] == a.ignore;
+    const T* const from = static_cast<const T*>(j.src) + r * j.ld + c;
+    T v[N] = {};
+    if (!out && c + N <= j.cols) {
+      typedef T any __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+      const any w = *reinterpret_cast<const any*>(from);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = w[e];
     } else if (!out) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (c + e < cols) v[e] = from[e];
+        if (c + e < j.cols) v[e] = from[e];
     }
-    unsigned char* const to = dst + r * pitch + (i - r * groups) * 16;
+    unsigned char* const to = j.dst + r * a.pitch + (i - r * groups) * 16;
     if constexpr (SPLIT) {
-      uint32_t p[3][4];
+      // (powers of two: the products are exact)
+      const float f = j.row_g ? inv_g * near_2_14(j.row_g[r]) : 1.f;
+      tu4 hi, lo;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float a = v[2 * q], b = v[2 * q + 1];
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          p[k][q] = bf16_pair(a, b);
-          a -= __builtin_bit_cast(float, p[k][q] << 16);
-          b -= __builtin_bit_cast(float, p[k][q] & 0xffff0000u);
-        }
+        const float x = v[2 * q] * inv * f, y = v[2 * q + 1] * inv * f;
+        hi[q] = f16_pair(x, y);
+        lo[q] = f16_pair(f16_rest(x), f16_rest(y));
       }
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        *reinterpret_cast<tu4*>(to + k * plane) = tu4{p[k][0], p[k][1], p[k][2], p[k][3]};
+      *reinterpret_cast<tu4*>(to) = hi;
+      *reinterpret_cast<tu4*>(to + plane) = lo;
     } else {
       typedef T whole __attribute__((ext_vector_type(N)));
       whole w;
@@ -113,7 +211,7 @@ struct ClassArgs {
   float* label_logit;              // [n]
   const cf2* stats;                // [n] (M, S)
   const float* g;                  // [n] upstream gradient
-  unsigned char* resid;            // r: [plane][n][ld] bfloat16
+  unsigned char* resid;            // r: [plane][n][pitch]
   int64_t resid_pitch, resid_plane;
   float* bias_part;                // [tiles_n][bias_ld], or NULL
   int64_t bias_ld;
@@ -121,16 +219,27 @@ struct ClassArgs {
   void* out;
   int64_t out_ld, out_split;       // elements; split s at out + s * out_split
   int out_bf16, accumulate;
+  // float32 as planes: what the accumulators count in is *scale_m * *scale_n of
+  // the operands' units; a row of r is in units of its own, near_2_14(g), which a
+  // product over the classes has in place of *scale_n (row_units)
+  const float *scale_m, *scale_n;
+  int row_units;
 };
+
+// how r is written
+template <int F32>
+using ResidAs = typename std::conditional<
+    F32 == 0, AsBf16, typename std::conditional<F32 == 1, AsF32, AsF16>::type>::type;
 
 // LDS behind the tile loop: what the epilogue exchanges; behind that the tile's
 // biases and their gradient's column sums
-template <typename C, int EPI>
-constexpr int kEpiLds = EPI == kEpiStats    ? C::WGM * C::BN * 8
-                        : EPI == kEpiResidual ? kTileRowsLds<C, uint16_t>
-                                              : kTileRowsLds<C, float>;
+template <typename C, int EPI, int F32>
+constexpr int kEpiLds = EPI == kEpiStats      ? C::WGM * C::BN * 8
+                        : EPI == kEpiResidual ? kTileRowsLds<C, ResidAs<F32>>
+                                              : kTileRowsLds<C, AsF32>;
 
-template <typename C, int EPI, bool F32>
+// F32: 0 bfloat16, 1 float32 as it is, 2 float32 in planes
+template <typename C, int EPI, int F32>
 __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_kernel(
     ClassArgs p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -193,21 +302,37 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
       for (int j = 0; j < C::WN; ++j) acc[i][j] = typename C::MMA::Acc{};
   }
 
+  // what an accumulator counts in: planes of scaled operands
+  float unit_m = 1.f, unit_n = 1.f;
+  float unit_r[C::WN];
+  if (F32 == 2) {
+    unit_m = *p.scale_m;
+    if (EPI != kEpiStore || !p.row_units) unit_n = *p.scale_n;
+    if (EPI != kEpiStats) {
+#pragma unroll
+      for (int j = 0; j < C::WN; ++j) {
+        const int64_t n = n0 + nw + j * 32 + col;
+        unit_r[j] = (EPI == kEpiResidual || p.row_units) && n < p.n ? near_2_14(p.g[n]) : 1.f;
+      }
+    }
+  }
   if constexpr (EPI == kEpiStore) {
     auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r) {
         v[r] = acc_get(acc[decltype(I)::value][decltype(J)::value], 4 * decltype(Q)::value + r);
+        if (F32 == 2) v[r] = v[r] * unit_m * unit_n * unit_r[decltype(J)::value];
+      }
     };
-    if (p.out_bf16) {
-      tile_rows<C, uint16_t>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+    if (F32 == 0 && p.out_bf16) {
+      tile_rows<C, AsBf16>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
         if (n0 + n < p.n && m0 + m < p.m)
           store_piece(static_cast<uint16_t*>(p.out) + (n0 + n) * p.out_ld + m0 + m,
                       p.m - m0 - m, piece);
       });
     } else {
       float* out = static_cast<float*>(p.out) + (int64_t)blockIdx.y * p.out_split;
-      tile_rows<C, float>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+      tile_rows<C, AsF32>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
         if (n0 + n >= p.n || m0 + m >= p.m) return;
         float* o = out + (n0 + n) * p.out_ld + m0 + m;
         tu4 sum = piece;
@@ -224,7 +349,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
     }
     return;
   } else {
-    float* sbias = reinterpret_cast<float*>(smem + kEpiLds<C, EPI>);
+    float* sbias = reinterpret_cast<float*>(smem + kEpiLds<C, EPI, F32>);
     // the lane's 16 WM classes' biases stay in registers (read per use, the LDS'
     // latency shows between the accumulator reads)
     tf4 bias[C::WM][4] = {};
@@ -241,7 +366,11 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
     auto logits = [&](auto I, auto J, auto Q, float (&l)[4]) {
       constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) l[r] = acc_get(acc[i][j], 4 * q + r) + bias[i][q][r];
+      for (int r = 0; r < 4; ++r) {
+        l[r] = acc_get(acc[i][j], 4 * q + r);
+        if (F32 == 2) l[r] = l[r] * unit_m * unit_n;
+        l[r] += bias[i][q][r];
+      }
     };
     auto blocks = [&](auto&& f) {
       tile_for<C::WM>([&](auto I) { tile_for<4>([&](auto Q) { f(I, Q); }); });
@@ -291,12 +420,12 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
         p.part[(int64_t)tm * p.n + n0 + i] = t;
       }
     } else {
-      // r, one plane at a time; the later planes of a float32 r compute it
-      // again rather than keep it
+      // r; of two planes one at a time, the second computing r again rather than
+      // keeping it
       float sum[C::WM][16];                // over the wave's rows, for the bias
       float* scol = sbias + C::BM;         // [WGN][BM]
 #pragma unroll 1
-      for (int pl = 0; pl < (F32 ? 3 : 1); ++pl) {
+      for (int pl = 0; pl < (F32 == 2 ? 2 : 1); ++pl) {
         if (pl) __syncthreads();           // the plane before has been read
         auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
           constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
@@ -312,16 +441,17 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
           }
-          if (F32) {
+          if (F32 == 2) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float v1 = v[r] - bf16_value(bf16_bits(v[r]));
-              v[r] = pl == 0 ? v[r] : pl == 1 ? v1 : v1 - bf16_value(bf16_bits(v1));
+              v[r] *= 1.f / unit_r[j];
+              v[r] = pl == 0 ? v[r] : f16_rest(v[r]);
             }
           }
         };
-        tile_rows<C, uint16_t>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
-          const int64_t byte = (m0 + m) * 2;
+        typedef ResidAs<F32> As;
+        tile_rows<C, As>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+          const int64_t byte = (m0 + m) * (int)sizeof(typename As::T);
           if (n0 + n < p.n && byte < p.resid_pitch)
             *reinterpret_cast<tu4*>(p.resid + pl * p.resid_plane + (n0 + n) * p.resid_pitch +
                                     byte) = piece;
@@ -406,7 +536,7 @@ __global__ void fill_kernel(uint16_t* __restrict__ out, int64_t n) {
 int64_t round_up(int64_t x, int64_t k) { return (x + k - 1) / k * k; }
 unsigned grid_for(int64_t items) {
   const int64_t b = (items + 255) / 256;
-  return (unsigned)(b < 1 ? 1 : b > 65536 ? 65536 : b);
+  return (unsigned)(b < 1 ? 1 : b > 16384 ? 16384 : b);
 }
 
 // bytes of r that one piece of classes may take: it is written, then read by
@@ -429,11 +559,11 @@ bool direct(const void* p, int64_t ld, const ClassProblem& q, bool whole) {
          (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * e <= kMaxPitch;
 }
 
-// Up to how many rows float32 operands are multiplied as they are, on
-// v_mfma_f32_32x32x2_f32 (2 N V D flop at 140 TFLOP/s), rather than packed into
-// planes (16 bytes an element of w, then six products at 1250): the two meet near
-// 770 rows.
-constexpr int64_t kWholeRows = 768;
+// Up to how many rows float32 operands are multiplied as they are, 2 N V D flop a
+// product at 140 TFLOP/s, rather than packed into planes: 12 bytes an element of w,
+// then three products at 1250.  They meet near 250 rows for the one product of the
+// forward call, near 80 for the three of the gradient's.
+constexpr int64_t kWholeRows = 256, kWholeRowsGrad = 80;
 
 // the logits' tiles: classes x rows of X
 constexpr int kTileClasses[] = {256, 128, 128, 128}, kTileRows[] = {256, 128, 64, 32};
@@ -443,7 +573,8 @@ struct ClassLayout {
   int64_t pitch;                   // of packed operands, bytes
   int64_t x_plane, w_plane, planes;
   bool pack_x, pack_w;
-  int64_t xp, wp;                  // offsets
+  int64_t xp, wp, xg;              // offsets; xg: X with its rows scaled like g's
+  int64_t maxima, scales;          // float32 in planes: of X, w, g
   int64_t part, label_logit;       // forward
   int tile;                        // see kTileClasses
   int64_t tiles_v;                 // parts of the statistics
@@ -459,8 +590,8 @@ int64_t tiles(int64_t n, int64_t b) { return (n + b - 1) / b; }
 
 ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   ClassLayout l;
-  l.whole = q.f32() && !grad && q.n <= kWholeRows;
-  l.planes = q.f32() && !l.whole ? 3 : 1;
+  l.whole = q.f32() && q.n <= (grad ? kWholeRowsGrad : kWholeRows);
+  l.planes = q.f32() && !l.whole ? 2 : 1;
   l.pitch = round_up(q.d * (l.whole ? 4 : 2), 128);
   l.pack_x = !direct(q.x, q.ldx, q, l.whole) || (grad && has_ignore);
   l.pack_w = !direct(q.w, q.ldw, q, l.whole);
@@ -473,11 +604,15 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     at += round_up(bytes, 1024);
     return here;
   };
+  l.maxima = l.planes > 1 ? take(3ll * kMaxParts * 4) : 0;
+  l.scales = l.planes > 1 ? take(3 * 4) : 0;
   l.xp = l.pack_x ? take(l.planes * l.x_plane) : 0;
   l.wp = l.pack_w ? take(l.planes * l.w_plane) : 0;
+  l.xg = grad && l.planes > 1 ? take(l.planes * l.x_plane) : 0;
+  const int64_t resid_bytes = q.f32() ? 4 : 2;
   l.piece = q.v;
   if (grad) {
-    int64_t c = kPieceBytes / (l.planes * 2 * (q.n > 0 ? q.n : 1)) / 256 * 256;
+    int64_t c = kPieceBytes / (resid_bytes * (q.n > 0 ? q.n : 1)) / 256 * 256;
     if (c < 4096) c = 4096;
     if (c < l.piece) l.piece = c;
   }
@@ -492,14 +627,14 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     l.part = take(l.tiles_v * q.n * 8);
     l.label_logit = take(q.n * 4);
   } else {
-    l.resid_pitch = round_up(l.piece, 64) * 2;
+    l.resid_pitch = round_up(l.piece * (l.whole ? 4 : 2), 128);
     l.resid_plane = q.n * l.resid_pitch;
     l.resid = take(l.planes * l.resid_plane);
     l.dw_tile = tiles(l.piece, 256) * tiles(q.d, 256) >= cus ? 0 : 1;
     l.dx_tile = tiles(q.n, 256) * tiles(q.d, 256) >= cus ? 0 : 1;
     const int64_t b = l.dx_tile == 0 ? 256 : 128;
     const int64_t t = tiles(q.n, b) * tiles(q.d, b);
-    const int64_t steps = tiles(l.piece, 64);
+    const int64_t steps = tiles(l.piece * (l.whole ? 4 : 2), 128);
     int64_t s = t > 0 ? (2 * cus) / t : 1;
     if (s > steps / 4) s = steps / 4;
     l.dx_splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -510,9 +645,9 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   return l;
 }
 
-template <typename C, int EPI, bool F32>
+template <typename C, int EPI, int F32>
 int launch_tile(const ClassArgs& a, hipStream_t s) {
-  constexpr int epi = kEpiLds<C, EPI> + C::BM * 4 * (1 + C::WGN);
+  constexpr int epi = kEpiLds<C, EPI, F32> + C::BM * 4 * (1 + C::WGN);
   constexpr int lds = C::kLds > epi ? C::kLds : epi;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   static thread_local int attr_dev = -1;
@@ -540,7 +675,7 @@ template <typename M, bool AK, bool BK> using Big = TileCfg<M, 2, 2, 4, 4, AK, B
 template <typename M, bool AK, bool BK> using Mid = TileCfg<M, 2, 2, 2, 2, AK, BK>;
 template <typename M, int WN> using Few = TileCfg<M, 4, 1, 1, WN, false, false>;
 
-template <typename M, int EPI, bool F32>
+template <typename M, int EPI, int F32>
 int launch_logits(const ClassArgs& a, int tile, hipStream_t s) {
   switch (tile) {
     case 0: return launch_tile<Big<M, false, false>, EPI, F32>(a, s);
@@ -550,45 +685,70 @@ int launch_logits(const ClassArgs& a, int tile, hipStream_t s) {
   }
 }
 
-int pack_rows(const void* src, int64_t rows, int64_t ld, const ClassProblem& q,
-              const ClassLayout& l, unsigned char* dst, int64_t plane, const int64_t* labels,
-              int64_t ignore, hipStream_t s) {
-  const dim3 grid(grid_for(rows * (l.pitch / 16)));
-  const float* f = static_cast<const float*>(src);
-  if (q.f32() && !l.whole)
-    hipLaunchKernelGGL((pack_rows_kernel<float, true>), grid, dim3(256), 0, s, f, rows, q.d, ld,
-                       dst, l.pitch, plane, labels, ignore);
-  else if (q.f32())
-    hipLaunchKernelGGL((pack_rows_kernel<float, false>), grid, dim3(256), 0, s, f, rows, q.d, ld,
-                       dst, l.pitch, plane, labels, ignore);
-  else
-    hipLaunchKernelGGL((pack_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s,
-                       static_cast<const uint16_t*>(src), rows, q.d, ld, dst, l.pitch, plane,
-                       labels, ignore);
-  ZS_LAUNCH_CHECK("pack_rows_kernel launch");
-  return ZSHMC_OK;
+// a product with r: k-major X and r (dw) or k-major w and rows of r (dX)
+template <bool BK, typename M, int F32>
+int launch_gradient_of(const ClassArgs& g, int tile, hipStream_t s) {
+  return tile == 0 ? launch_tile<Big<M, true, BK>, kEpiStore, F32>(g, s)
+                   : launch_tile<Mid<M, true, BK>, kEpiStore, F32>(g, s);
+}
+template <bool BK>
+int launch_gradient(const ClassArgs& g, const ClassLayout& l, int tile, hipStream_t s) {
+  return l.planes > 1 ? launch_gradient_of<BK, MmaF16, 2>(g, tile, s)
+         : l.whole    ? launch_gradient_of<BK, MmaF32, 1>(g, tile, s)
+                      : launch_gradient_of<BK, MmaBf16, 0>(g, tile, s);
 }
 
-// the operands X and w, packed where they have to be
+// The operands X and w, packed where they have to be; `labels`: rows of X that are
+// ignored are left out (NULL: none).  With `g`, xg is X as the product with r over
+// the rows takes it: in planes, a row of r is in units of its own, which its row
+// of X makes up for.
 int operands(const ClassProblem& q, const ClassLayout& l, unsigned char* ws,
-             const int64_t* drop_labels, int64_t ignore, hipStream_t s, TileOperand* x,
-             TileOperand* w) {
-  const unsigned char* px = static_cast<const unsigned char*>(q.x);
-  const unsigned char* pw = static_cast<const unsigned char*>(q.w);
+             const int64_t* labels, int64_t ignore, const float* g, hipStream_t s, TileOperand* x,
+             TileOperand* w, TileOperand* xg) {
   const int64_t e = q.esize();
-  *x = TileOperand{px, q.ldx * e, 0, q.n, q.d * e};
-  *w = TileOperand{pw, q.ldw * e, 0, q.v, q.d * e};
-  if (l.pack_x) {
-    const int rc = pack_rows(q.x, q.n, q.ldx, q, l, ws + l.xp, l.x_plane, drop_labels, ignore,
-                             s);
-    if (rc != ZSHMC_OK) return rc;
-    *x = TileOperand{ws + l.xp, l.pitch, l.x_plane, q.n, l.pitch};
+  *x = TileOperand{static_cast<const unsigned char*>(q.x), q.ldx * e, 0, q.n, q.d * e};
+  *w = TileOperand{static_cast<const unsigned char*>(q.w), q.ldw * e, 0, q.v, q.d * e};
+  const PackJob jx{q.x, q.n, q.d, q.ldx, ws + l.xp, labels, nullptr, 0, g ? 2 : 0, 1};
+  const PackJob jw{q.w, q.v, q.d, q.ldw, ws + l.wp, nullptr, nullptr, 1, 1, 1};
+  PackJob jg = jx;
+  jg.dst = ws + l.xg;
+  jg.row_g = g;
+  jg.part_g = 2;
+  jg.writes = 0;
+  const TileOperand px{ws + l.xp, l.pitch, l.x_plane, q.n, l.pitch};
+  const TileOperand pw{ws + l.wp, l.pitch, l.w_plane, q.v, l.pitch};
+  PackArgs a{};
+  a.pitch = l.pitch;
+  a.ignore = ignore;
+  a.part = reinterpret_cast<const float*>(ws + l.maxima);
+  a.scale = reinterpret_cast<float*>(ws + l.scales);
+  int jobs = 0;
+  int64_t most = 0;
+  auto add = [&](const PackJob& j) {
+    a.job[jobs++] = j;
+    if (j.rows > most) most = j.rows;
+  };
+  if (l.pack_x) add(jx), *x = px;
+  if (l.pack_w) add(jw), *w = pw;
+  if (xg) *xg = *x;
+  if (l.planes > 1) {                      // (both are packed)
+    if (xg) {
+      add(jg);
+      xg->base = ws + l.xg;
+    }
+    hipLaunchKernelGGL(part_max_kernel, dim3(kMaxParts, 3), dim3(256), 0, s, a, g,
+                       reinterpret_cast<float*>(ws + l.maxima));
+    ZS_LAUNCH_CHECK("part_max_kernel launch");
   }
-  if (l.pack_w) {
-    const int rc = pack_rows(q.w, q.v, q.ldw, q, l, ws + l.wp, l.w_plane, nullptr, 0, s);
-    if (rc != ZSHMC_OK) return rc;
-    *w = TileOperand{ws + l.wp, l.pitch, l.w_plane, q.v, l.pitch};
-  }
+  if (!jobs) return ZSHMC_OK;
+  const dim3 grid(grid_for(most * (l.pitch / 16)), (unsigned)jobs);
+  if (l.planes > 1)
+    hipLaunchKernelGGL((pack_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
+  else if (q.f32())
+    hipLaunchKernelGGL((pack_rows_kernel<float, false>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((pack_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s, a);
+  ZS_LAUNCH_CHECK("pack_rows_kernel launch");
   return ZSHMC_OK;
 }
 
@@ -658,18 +818,22 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   ClassArgs a{};
   a.part = reinterpret_cast<cf2*>(ws + l.part);
   a.label_logit = reinterpret_cast<float*>(ws + l.label_logit);
-  rc = operands(q, l, ws, nullptr, 0, s, &a.b, &a.a);
+  rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, nullptr, s, &a.b, &a.a,
+                nullptr);
   if (rc != ZSHMC_OK) return rc;
   a.m = q.v;
   a.n = q.n;
   a.steps = (int)tiles(q.d * (l.whole ? 4 : 2), 128);
-  a.terms = l.planes > 1 ? kTerms3 : 1;
+  a.terms = l.planes > 1 ? kTermsSplit : 1;
+  a.scale_n = reinterpret_cast<const float*>(ws + l.scales);
+  a.scale_m = a.scale_n + 1;
   a.splits = 1;
   a.bias = bias;
   a.labels = labels;
   a.n_classes = q.v;
-  rc = l.whole ? launch_logits<MmaF32, kEpiStats, false>(a, l.tile, s)
-               : launch_logits<MmaBf16, kEpiStats, false>(a, l.tile, s);
+  rc = l.planes > 1 ? launch_logits<MmaF16, kEpiStats, 2>(a, l.tile, s)
+       : l.whole    ? launch_logits<MmaF32, kEpiStats, 1>(a, l.tile, s)
+                    : launch_logits<MmaBf16, kEpiStats, 0>(a, l.tile, s);
   if (rc != ZSHMC_OK) return rc;
   return join_stats(q, l, a, labels, has_ignore, ignore_label, log_prob, stats, s);
 }
@@ -703,23 +867,28 @@ extern "C" int zshmc_class_log_prob_grad(
              "zshmc_class_log_prob_grad: %lld bytes of 16-byte aligned workspace needed, got "
              "%lld", (long long)l.total, (long long)workspace_bytes);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  TileOperand ox, ow;
-  rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, s, &ox, &ow);
+  TileOperand ox, ow, og;
+  rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, grad_log_prob, s, &ox,
+                &ow, &og);
   if (rc != ZSHMC_OK) return rc;
-  const int terms = q.f32() ? kTerms3 : 1;
+  const int terms = l.planes > 1 ? kTermsSplit : 1;
+  const int64_t pb = l.whole ? 4 : 2;            // bytes of a plane's element
+  const float* scales = reinterpret_cast<const float*>(ws + l.scales);
   for (int64_t c0 = 0; c0 < q.v; c0 += l.piece) {
     const int64_t c = q.v - c0 < l.piece ? q.v - c0 : l.piece;
     TileOperand wp = ow;
     wp.base += c0 * wp.pitch;
     wp.rows = c;
-    const TileOperand r{ws + l.resid, l.resid_pitch, l.resid_plane, q.n, round_up(c, 64) * 2};
+    const TileOperand r{ws + l.resid, l.resid_pitch, l.resid_plane, q.n, round_up(c * pb, 128)};
     ClassArgs a{};
     a.a = wp;
     a.b = ox;
     a.m = c;
     a.n = q.n;
-    a.steps = (int)tiles(q.d, 64);
+    a.steps = (int)tiles(q.d * pb, 128);
     a.terms = terms;
+    a.scale_n = scales;
+    a.scale_m = scales + 1;
     a.splits = 1;
     a.bias = bias ? bias + c0 : nullptr;
     a.labels = labels;
@@ -734,23 +903,25 @@ extern "C" int zshmc_class_log_prob_grad(
     a.resid_plane = l.resid_plane;
     a.bias_part = grad_bias ? reinterpret_cast<float*>(ws + l.bias_part) : nullptr;
     a.bias_ld = q.v;
-    rc = q.f32() ? launch_logits<MmaBf16, kEpiResidual, true>(a, l.tile, s)
-                 : launch_logits<MmaBf16, kEpiResidual, false>(a, l.tile, s);
+    rc = l.planes > 1 ? launch_logits<MmaF16, kEpiResidual, 2>(a, l.tile, s)
+         : l.whole    ? launch_logits<MmaF32, kEpiResidual, 1>(a, l.tile, s)
+                      : launch_logits<MmaBf16, kEpiResidual, 0>(a, l.tile, s);
     if (rc != ZSHMC_OK) return rc;
     if (grad_w) {                  // dw = r^T X over the rows of X
       ClassArgs g{};
-      g.a = ox;
+      g.a = og;
       g.b = r;
       g.m = q.d;
       g.n = c;
-      g.steps = (int)tiles(q.n, 64);
+      g.steps = (int)tiles(q.n * pb, 128);
       g.terms = terms;
+      g.scale_m = scales;
+      g.scale_n = scales + 2;
       g.splits = 1;
       g.out = static_cast<unsigned char*>(grad_w) + c0 * q.d * q.esize();
       g.out_ld = q.d;
       g.out_bf16 = !q.f32();
-      rc = l.dw_tile == 0 ? launch_tile<Big<MmaBf16, true, true>, kEpiStore, false>(g, s)
-                          : launch_tile<Mid<MmaBf16, true, true>, kEpiStore, false>(g, s);
+      rc = launch_gradient<true>(g, l, l.dw_tile, s);
       if (rc != ZSHMC_OK) return rc;
     }
     if (grad_x) {                  // dX += r w over the piece's classes
@@ -759,15 +930,17 @@ extern "C" int zshmc_class_log_prob_grad(
       g.b = r;
       g.m = q.d;
       g.n = q.n;
-      g.steps = (int)tiles(c, 64);
+      g.steps = (int)tiles(c * pb, 128);
       g.terms = terms;
+      g.scale_m = scales + 1;
+      g.g = grad_log_prob;
+      g.row_units = 1;
       g.splits = l.dx_splits;
       g.out = ws + l.dx_part;
       g.out_ld = q.d;
       g.out_split = q.n * q.d;
       g.accumulate = c0 > 0;
-      rc = l.dx_tile == 0 ? launch_tile<Big<MmaBf16, true, false>, kEpiStore, false>(g, s)
-                          : launch_tile<Mid<MmaBf16, true, false>, kEpiStore, false>(g, s);
+      rc = launch_gradient<false>(g, l, l.dx_tile, s);
       if (rc != ZSHMC_OK) return rc;
     }
   }

@@ -284,8 +284,9 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void int8_tile_ke
   }
   ti16 acc[C::WM][C::WN];
   tile_loop<C>(p.a, p.b, m0, n0, 0, p.steps, 1, lds, lane, wave, acc);
-  typedef typename std::conditional<BF16, uint16_t, float>::type T;
-  float* ssw = reinterpret_cast<float*>(smem + kTileRowsLds<C, T>);     // [2][BM]
+  typedef typename std::conditional<BF16, AsBf16, AsF32>::type As;
+  typedef typename As::T T;
+  float* ssw = reinterpret_cast<float*>(smem + kTileRowsLds<C, As>);    // [2][BM]
   if (threadIdx.x < C::BM) {
     ssw[threadIdx.x] = sw_here;
     ssw[C::BM + threadIdx.x] = bias_here;
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void int8_tile_ke
     for (int r = 0; r < 4; ++r)
       v[r] = (float)acc_get(acc[i][j], 4 * q + r) * (sx[j] * sw[i][q][r]) + bias[i][q][r];
   };
-  tile_rows<C, T>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+  tile_rows<C, As>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
     if (n0 + n < p.n && m0 + m < p.m)
       store_piece(static_cast<T*>(p.out) + (n0 + n) * p.ldo + m0 + m, p.m - m0 - m, piece);
   });
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void int8_tile_ke
 template <typename C, bool BF16>
 int launch_int8(const Int8Args& a, hipStream_t s) {
   constexpr int epi =
-      kTileRowsLds<C, typename std::conditional<BF16, uint16_t, float>::type> + C::BM * 8;
+      kTileRowsLds<C, typename std::conditional<BF16, AsBf16, AsF32>::type> + C::BM * 8;
   constexpr int lds = C::kLds > epi ? C::kLds : epi;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   static thread_local int attr_dev = -1;

@@ -11,11 +11,12 @@
 //     bytes; its eight 16-byte chunks are rotated by XOR with (m >> 1) & 7, so
 //     that the 16 lanes that a ds_read_b128 serves at a time (rows {0-3, 12-15,
 //     20-27} / {4-11, 16-19, 28-31} of a 32-row block) touch all 64 banks once.
-//   k-major ("km", 2-byte elements): row k holds the m's side by side.  The LDS
-//     row k is BM (BN) elements and the fragment is taken by the transposing
+//   k-major ("km"): row k holds the m's side by side.  The LDS row k is BM (BN)
+//     elements.  2-byte elements: the fragment is taken by the transposing
 //     read ds_read_b64_tr_b16, 4 k's x 16 m's per group of 16 lanes; chunks are
 //     XORed with 4 (k & 3) so that the four k rows of a read sit in different
-//     quarters of the banks.  The gradient products contract over rows this
+//     quarters of the banks.  4-byte elements: four ds_read_b32, the lane
+//     halves' rows (4 apart) in different halves of the banks by XOR with 8.  The gradient products contract over rows this
 //     way and no operand is ever transposed in memory.
 // A step's four MFMA k-slices (kk) are software-pipelined over two register
 // sets; the one barrier of a step sits in front of its LAST slice, whose
@@ -31,10 +32,11 @@
 // 1385; eight waves of 128 x 64 each 1345, 64-byte steps in four buffers 1280,
 // two workgroups of 128 x 128 a CU 1105.
 //
-// `terms`: float32 operands come as three bfloat16 planes (x = hi + mid + lo,
-// exact) and a product is the six plane pairs whose weight is above 2^-24:
-// the loop runs over the pairs, smallest first, into the same float32
-// accumulators.  One pair otherwise.
+// `terms`: float32 operands may come as two float16 planes of x / 2^e, hi and lo =
+// the rest (22 bits and a sign; 2^e an operand's own, its largest magnitude near
+// 2^14, so that what float16 cannot hold is 2^-38 of that), and a product is hi lo
+// + lo hi + hi hi: what is left out is 2^-22 of it.  The loop runs over the pairs,
+// smallest first, into the same float32 accumulators.  One pair otherwise.
 #pragma once
 #include <type_traits>
 #include <utility>
@@ -51,6 +53,7 @@ typedef float tf4 __attribute__((ext_vector_type(4)));
 typedef float tf16 __attribute__((ext_vector_type(16)));
 typedef int ti16 __attribute__((ext_vector_type(16)));
 typedef __bf16 tb8 __attribute__((ext_vector_type(8)));
+typedef _Float16 th8 __attribute__((ext_vector_type(8)));
 #define ZS_TLDS __attribute__((address_space(3)))
 
 // One operand as it lies in memory: rows x row_bytes, `pitch` bytes apart
@@ -61,11 +64,10 @@ struct TileOperand {
   int64_t rows, row_bytes;
 };
 
-// plane pairs, two bits each, smallest product first; bf16 / int8 use pair 0
-// of one term (hi x hi)
-constexpr int kTerms3 = 6;
-constexpr uint32_t kTermsA3 = 1u | 2u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
-constexpr uint32_t kTermsB3 = 1u | 0u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+// plane pairs, two bits each, smallest products first (one term: pair 0 0)
+constexpr int kTermsSplit = 3;
+constexpr uint32_t kTermsA = 0u | 1u << 2 | 0u << 4;
+constexpr uint32_t kTermsB = 1u | 0u << 2 | 0u << 4;
 
 // two float32 -> bfloat16 (to nearest even) in one register
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
@@ -74,17 +76,34 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   return __builtin_bit_cast(uint32_t, p);
 }
 
+__device__ __forceinline__ uint32_t f16_pair(float a, float b) {
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  const pair p = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(uint32_t, p);
+}
+
+// kBytes: of an element of a k-major operand
 struct MmaBf16 {
   typedef tf16 Acc;
+  static constexpr int kBytes = 2;
   static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
         __builtin_bit_cast(tb8, a), __builtin_bit_cast(tb8, b), c, 0, 0, 0);
+  }
+};
+struct MmaF16 {
+  typedef tf16 Acc;
+  static constexpr int kBytes = 2;
+  static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(th8, a), __builtin_bit_cast(th8, b), c, 0, 0, 0);
   }
 };
 // float32 as it is: a lane's four elements of a chunk one MFMA each (k is a dummy
 // index; both operands hold the same four)
 struct MmaF32 {
   typedef tf16 Acc;
+  static constexpr int kBytes = 4;
   static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, Acc c) {
     const tf4 x = __builtin_bit_cast(tf4, a), y = __builtin_bit_cast(tf4, b);
 #pragma unroll
@@ -95,6 +114,7 @@ struct MmaF32 {
 };
 struct MmaI8 {
   typedef ti16 Acc;
+  static constexpr int kBytes = 1;
   static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(
         __builtin_bit_cast(ti4, a), __builtin_bit_cast(ti4, b), c, 0, 0, 0);
@@ -151,9 +171,10 @@ struct TileCfg {
 
 // One operand's side of a step: its DMA lane offsets and its LDS fragments.
 // ROWS: BM or BN; OFF: its place in a stage; NB: 32-blocks of the wave.
-template <bool KM, int ROWS, int OFF, int NB>
+template <bool KM, int ROWS, int OFF, int NB, int ES>
 struct TileSide {
   static constexpr int kPieces = ROWS / 8 / 4;     // 1 KB pieces per wave
+  static constexpr int kStepRows = 128 / ES;       // km: rows of a step
   uint32_t voff[kPieces];
   uint32_t chunk16;          // kc: the lane's chunk offset within 128 bytes
   uint32_t frag[KM ? NB : 4];
@@ -190,25 +211,27 @@ struct TileSide {
       for (int kk = 0; kk < 4; ++kk)
         frag[kk] = r + (uint32_t)(((2 * kk + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16);
     } else {
-      constexpr int CR = ROWS / 8;                 // chunks per LDS row
+      constexpr int CR = ROWS * ES / 16;           // chunks per LDS row
       constexpr int RP = 64 / CR;                  // rows per piece
-      const int sub = lane / CR;
-      const int row3 = (RP * wave + sub) & 3;
-      const uint32_t c = (uint32_t)((lane % CR) ^ (4 * row3));
       chunk16 = 0;
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j)
-        voff[j] = (uint32_t)((RP * (wave + 4 * j) + sub) * pitch) + c * 16;
-      at = (int64_t)k0 * 64 * pitch + row0 * 2;
+      for (int j = 0; j < kPieces; ++j) {
+        const int row = RP * (wave + 4 * j) + lane / CR;
+        const int swap = ES == 2 ? 4 * (row & 3) : 8 * ((row >> 2) & 1);
+        voff[j] = (uint32_t)(row * pitch) + (uint32_t)((lane % CR) ^ swap) * 16;
+      }
+      at = (int64_t)k0 * kStepRows * pitch + row0 * ES;
       end = (o.rows - 1) * pitch + o.row_bytes;
       left = 0;
-      step_bytes = 64 * pitch;
-      const int k3 = (lane & 15) >> 2;
-      const uint32_t kr = OFF + (uint32_t)(((lane >> 5) * 8 + k3) * (ROWS * 2)) + (lane & 1) * 8;
+      step_bytes = kStepRows * pitch;
+      const int k3 = (lane & 15) >> 2, half = lane >> 5;
+      const uint32_t kr = OFF + (ES == 2 ? (uint32_t)((half * 8 + k3) * (ROWS * 2) + (lane & 1) * 8)
+                                         : (uint32_t)(half * 4 * (ROWS * 4) + (lane & 3) * 4));
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const int ch = (blk0 + b) * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-        frag[b] = kr + (uint32_t)((ch ^ (4 * k3)) * 16);
+        const int ch = ES == 2 ? (blk0 + b) * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)
+                               : (blk0 + b) * 8 + ((lane & 31) >> 2);
+        frag[b] = kr + (uint32_t)((ch ^ (ES == 2 ? 4 * k3 : 8 * half)) * 16);
       }
     }
     plane = o.plane;
@@ -261,6 +284,11 @@ struct TileSide {
     if constexpr (!KM) {
       f = *reinterpret_cast<const ZS_TLDS tu4*>(
           (uintptr_t)(stage + frag[kk] + (uint32_t)(b * 4096)));
+    } else if constexpr (ES == 4) {
+      const uint32_t at = stage + frag[b] + (uint32_t)(kk * 8 * ROWS * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f[e] = *reinterpret_cast<const ZS_TLDS uint32_t*>((uintptr_t)(at + e * ROWS * 4));
     } else {
       const uint32_t at = stage + frag[b] + (uint32_t)(kk * 16 * ROWS * 2);
       const tu2 lo = __builtin_bit_cast(
@@ -281,14 +309,14 @@ __device__ __forceinline__ void tile_loop(const TileOperand& A, const TileOperan
                                           int64_t m0, int64_t n0, int k0, int steps, int terms,
                                           uint32_t lds, int lane, int wave,
                                           typename C::MMA::Acc (&acc)[C::WM][C::WN]) {
-  typedef TileSide<C::A_KM, C::BM, 0, C::WM> SideA;
-  typedef TileSide<C::B_KM, C::BN, 3 * C::BM * 128, C::WN> SideB;
+  typedef TileSide<C::A_KM, C::BM, 0, C::WM, C::MMA::kBytes> SideA;
+  typedef TileSide<C::B_KM, C::BN, 3 * C::BM * 128, C::WN, C::MMA::kBytes> SideB;
   constexpr int PA = SideA::kPieces, PB = SideB::kPieces;
   constexpr int M = C::WM * C::WN, R = C::WM + C::WN;
   SideA sa;
   SideB sb;
-  sa.init(A, m0, k0, lane, wave, (wave / C::WGN) * C::WM, terms > 1 ? kTermsA3 : 0u);
-  sb.init(B, n0, k0, lane, wave, (wave % C::WGN) * C::WN, terms > 1 ? kTermsB3 : 0u);
+  sa.init(A, m0, k0, lane, wave, (wave / C::WGN) * C::WM, terms > 1 ? kTermsA : 0u);
+  sb.init(B, n0, k0, lane, wave, (wave % C::WGN) * C::WN, terms > 1 ? kTermsB : 0u);
 #pragma unroll
   for (int i = 0; i < C::WM; ++i)
 #pragma unroll
@@ -421,13 +449,33 @@ __device__ __forceinline__ int acc_get(const ti16& v, int r) {
 // WGN x 32 rows of BM values are written as elements T (float, or bfloat16 bits),
 // 16 bytes between rows so that they start in different banks, and read back
 // in 16-byte pieces; two regions alternate, one barrier a block column.
+// As: how a value is written (AsF32, AsBf16, AsF16).
 //   value(i, j, q, v): the four values of registers 4 q .. 4 q + 3 of block (i, j)
 //   emit(n, m, piece): 16 bytes of row n (of the tile) from column m on
-template <typename C, typename T>
-constexpr int kTileRowsLds = 2 * C::WGN * 32 * (C::BM * (int)sizeof(T) + 16);
+struct AsF32 {
+  typedef float T;
+  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
+    *reinterpret_cast<tf4*>(to) = tf4{v[0], v[1], v[2], v[3]};
+  }
+};
+struct AsBf16 {
+  typedef uint16_t T;
+  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
+    *reinterpret_cast<tu2*>(to) = tu2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+  }
+};
+struct AsF16 {
+  typedef uint16_t T;
+  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
+    *reinterpret_cast<tu2*>(to) = tu2{f16_pair(v[0], v[1]), f16_pair(v[2], v[3])};
+  }
+};
+template <typename C, typename As>
+constexpr int kTileRowsLds = 2 * C::WGN * 32 * (C::BM * (int)sizeof(typename As::T) + 16);
 
-template <typename C, typename T, typename V, typename E>
+template <typename C, typename As, typename V, typename E>
 __device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& value, E&& emit) {
+  typedef typename As::T T;
   constexpr int kRows = C::WGN * 32, kPitch = C::BM * (int)sizeof(T) + 16;
   constexpr int kPer = 16 / (int)sizeof(T), kPieces = C::BM / kPer;
   const int half = lane >> 5, col = lane & 31;
@@ -442,11 +490,7 @@ __device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& va
         constexpr int q = decltype(Q)::value;
         float v[4];
         value(I, J, Q, v);
-        char* to = mine + region + (i * 32 + 8 * q) * (int)sizeof(T);
-        if constexpr (sizeof(T) == 4)
-          *reinterpret_cast<tf4*>(to) = tf4{v[0], v[1], v[2], v[3]};
-        else
-          *reinterpret_cast<tu2*>(to) = tu2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+        As::put(mine + region + (i * 32 + 8 * q) * (int)sizeof(T), v);
       });
     });
     __syncthreads();

@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
   // first (or -1), M, g and -g / S
   int yl[C::WN];
   float mx[C::WN], g[C::WN], ginv[C::WN], bias_here = 0.f;
-  const bool biased = EPI != kEpiStore && (p.bias || m0 + C::BM > p.m);
+  const bool biased = EPI != kEpiStore && (p.bias || p.bias_part || m0 + C::BM > p.m);
   if constexpr (EPI != kEpiStore) {
 #pragma unroll
     for (int j = 0; j < C::WN; ++j) {
@@ -363,54 +363,62 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
           bias[i][q] = *reinterpret_cast<const tf4*>(sbias + mw + 4 * half + i * 32 + 8 * q);
     }
     // the logits of registers 4 q .. 4 q + 3 of block (i, j)
-    auto logits = [&](auto I, auto J, auto Q, float (&l)[4]) {
+    auto logits = [&](auto I, auto J, auto Q, auto BIASED, float (&l)[4]) {
       constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         l[r] = acc_get(acc[i][j], 4 * q + r);
         if (F32 == 2) l[r] = l[r] * unit_m * unit_n;
-        l[r] += bias[i][q][r];
+        if (decltype(BIASED)::value) l[r] += bias[i][q][r];
       }
     };
     auto blocks = [&](auto&& f) {
       tile_for<C::WM>([&](auto I) { tile_for<4>([&](auto Q) { f(I, Q); }); });
     };
+    // is some row's label in the wave's classes?
+    bool near[C::WN];
+#pragma unroll
+    for (int j = 0; j < C::WN; ++j) near[j] = __any(yl[j] >= 0);
     if constexpr (EPI == kEpiStats) {
       cf2* red = reinterpret_cast<cf2*>(smem);               // [WGM][BN]
-      tile_for<C::WN>([&](auto J) {
-        constexpr int j = decltype(J)::value;
-        float most = -__builtin_inff();
-        blocks([&](auto I, auto Q) {
-          float l[4];
-          logits(I, J, Q, l);
-          most = fmaxf(fmaxf(most, fmaxf(l[0], l[1])), fmaxf(l[2], l[3]));
-        });
-        if (__any(yl[j] >= 0)) {           // some row's label is in these classes
-          float picked = 0.f;
+      auto sweep = [&](auto BIASED) {
+        tile_for<C::WN>([&](auto J) {
+          constexpr int j = decltype(J)::value;
+          float l[C::WM][4][4];            // one read of the accumulators
+          float most = -__builtin_inff();
           blocks([&](auto I, auto Q) {
-            constexpr int i = decltype(I)::value, q = decltype(Q)::value;
-            float l[4];
-            logits(I, J, Q, l);
+            float(&v)[4] = l[decltype(I)::value][decltype(Q)::value];
+            logits(I, J, Q, BIASED, v);
+            most = fmaxf(fmaxf(most, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
+          });
+          if (near[j]) {
+            float picked = 0.f;
+            blocks([&](auto I, auto Q) {
+              constexpr int i = decltype(I)::value, q = decltype(Q)::value;
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (yl[j] == i * 32 + acc_row(4 * q + r, half)) picked = l[i][q][r];
+            });
+            if (yl[j] >= 0 && ((yl[j] >> 2) & 1) == half)
+              p.label_logit[n0 + nw + j * 32 + col] = picked;
+          }
+          most = fmaxf(most, __shfl_xor(most, 32, 64));
+          const float off = most == -__builtin_inff() ? 0.f : most;
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+          blocks([&](auto I, auto Q) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (yl[j] == i * 32 + acc_row(4 * q + r, half)) picked = l[r];
+              s[r] += fast_exp(l[decltype(I)::value][decltype(Q)::value][r] - off);
           });
-          if (yl[j] >= 0 && ((yl[j] >> 2) & 1) == half)
-            p.label_logit[n0 + nw + j * 32 + col] = picked;
-        }
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const float off = most == -__builtin_inff() ? 0.f : most;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        blocks([&](auto I, auto Q) {
-          float l[4];
-          logits(I, J, Q, l);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[r] += fast_exp(l[r] - off);
+          float sum = (s[0] + s[1]) + (s[2] + s[3]);
+          sum += __shfl_xor(sum, 32, 64);
+          if (half == 0) red[wm * C::BN + nw + j * 32 + col] = cf2{most, sum};
         });
-        float sum = (s[0] + s[1]) + (s[2] + s[3]);
-        sum += __shfl_xor(sum, 32, 64);
-        if (half == 0) red[wm * C::BN + nw + j * 32 + col] = cf2{most, sum};
-      });
+      };
+      if (biased)
+        sweep(std::true_type{});
+      else
+        sweep(std::false_type{});
       __syncthreads();
       for (int i = threadIdx.x; i < C::BN; i += 256) {
         if (n0 + i >= p.n) continue;
@@ -427,35 +435,41 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll 1
       for (int pl = 0; pl < (F32 == 2 ? 2 : 1); ++pl) {
         if (pl) __syncthreads();           // the plane before has been read
-        auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
-          constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
-          logits(I, J, Q, v);
+        auto write = [&](auto BIASED) {
+          auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
+            constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
+            logits(I, J, Q, BIASED, v);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = ginv[j] * fast_exp(v[r] - mx[j]);
-          if (__any(yl[j] >= 0)) {
+            for (int r = 0; r < 4; ++r) v[r] = ginv[j] * fast_exp(v[r] - mx[j]);
+            if (near[j]) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (yl[j] == i * 32 + acc_row(4 * q + r, half)) v[r] += g[j];
-          }
-          if (pl == 0 && p.bias_part) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
-          }
-          if (F32 == 2) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              v[r] *= 1.f / unit_r[j];
-              v[r] = pl == 0 ? v[r] : f16_rest(v[r]);
+              for (int r = 0; r < 4; ++r)
+                if (yl[j] == i * 32 + acc_row(4 * q + r, half)) v[r] += g[j];
             }
-          }
+            if (decltype(BIASED)::value && pl == 0 && p.bias_part) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
+            }
+            if (F32 == 2) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                v[r] *= 1.f / unit_r[j];
+                v[r] = pl == 0 ? v[r] : f16_rest(v[r]);
+              }
+            }
+          };
+          typedef ResidAs<F32> As;
+          tile_rows<C, As>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+            const int64_t byte = (m0 + m) * (int)sizeof(typename As::T);
+            if (n0 + n < p.n && byte < p.resid_pitch)
+              *reinterpret_cast<tu4*>(p.resid + pl * p.resid_plane + (n0 + n) * p.resid_pitch +
+                                      byte) = piece;
+          });
         };
-        typedef ResidAs<F32> As;
-        tile_rows<C, As>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
-          const int64_t byte = (m0 + m) * (int)sizeof(typename As::T);
-          if (n0 + n < p.n && byte < p.resid_pitch)
-            *reinterpret_cast<tu4*>(p.resid + pl * p.resid_plane + (n0 + n) * p.resid_pitch +
-                                    byte) = piece;
-        });
+        if (biased)
+          write(std::true_type{});
+        else
+          write(std::false_type{});
         if (pl == 0 && p.bias_part) {
           blocks([&](auto I, auto Q) {
             constexpr int i = decltype(I)::value, q = decltype(Q)::value;
@@ -617,10 +631,11 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     if (c < l.piece) l.piece = c;
   }
   l.pieces = tiles(q.v, l.piece);
-  // large tiles where they fill the chip
+  const int64_t element = l.whole ? 4 : 2, terms = l.planes > 1 ? kTermsSplit : 1;
   l.tile = q.n <= 32                                            ? 3
            : q.n <= 64                                          ? 2
-           : tiles(l.piece, 256) * tiles(q.n, 256) >= cus ? 0 : 1;
+           : plan_tiles(l.piece, q.n, terms * tiles(q.d * element, 128), false, cus).big ? 0
+                                                                                         : 1;
   l.tiles_v = tiles(q.v, kTileClasses[l.tile]);
   l.part = l.label_logit = l.resid = l.dx_part = l.bias_part = 0;
   if (!grad) {
@@ -630,14 +645,12 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     l.resid_pitch = round_up(l.piece * (l.whole ? 4 : 2), 128);
     l.resid_plane = q.n * l.resid_pitch;
     l.resid = take(l.planes * l.resid_plane);
-    l.dw_tile = tiles(l.piece, 256) * tiles(q.d, 256) >= cus ? 0 : 1;
-    l.dx_tile = tiles(q.n, 256) * tiles(q.d, 256) >= cus ? 0 : 1;
-    const int64_t b = l.dx_tile == 0 ? 256 : 128;
-    const int64_t t = tiles(q.n, b) * tiles(q.d, b);
-    const int64_t steps = tiles(l.piece * (l.whole ? 4 : 2), 128);
-    int64_t s = t > 0 ? (2 * cus) / t : 1;
-    if (s > steps / 4) s = steps / 4;
-    l.dx_splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    l.dw_tile = plan_tiles(l.piece, q.d, terms * tiles(q.n * element, 128), false, cus).big ? 0
+                                                                                            : 1;
+    const TilePlan dx = plan_tiles(q.n, q.d, terms * tiles(l.piece * element, 128), true, cus);
+    l.dx_tile = dx.big ? 0 : 1;
+    const int64_t steps = tiles(l.piece * element, 128);
+    l.dx_splits = (int)(dx.splits < steps ? dx.splits : steps);
     l.dx_part = take(l.dx_splits * q.n * q.d * 4);
     l.bias_part = take(tiles(q.n, kTileRows[l.tile]) * q.v * 4);
   }
@@ -756,8 +769,8 @@ int join_stats(const ClassProblem& q, const ClassLayout& l, const ClassArgs& a,
                const int64_t* labels, int has_ignore, int64_t ignore, float* log_prob,
                float* stats, hipStream_t s) {
   cf2* st = reinterpret_cast<cf2*>(stats);
-  // a workgroup per row where 16 rows a workgroup leave the chip empty
-  if (q.n <= 16ll * device_cu_count())
+  // two rows a workgroup where 16 leave the chip empty
+  if (q.n <= 4ll * device_cu_count())
     hipLaunchKernelGGL(join_stats_kernel<2>, dim3((unsigned)tiles(q.n, 2)), dim3(256), 0, s,
                        a.part, (int)l.tiles_v, a.label_logit, labels, q.n, q.v, has_ignore,
                        ignore, log_prob, st);

@@ -415,8 +415,7 @@ int product(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t
   a.ldo = ldo;
   if (n_rows <= 32)
     return bf16 ? launch_int8<FewI8, true>(a, s) : launch_int8<FewI8, false>(a, s);
-  const int64_t big = ((n_rows + 255) / 256) * ((n_channels + 255) / 256);
-  if (big >= device_cu_count())
+  if (plan_tiles(n_channels, n_rows, a.steps, false, device_cu_count()).big)
     return bf16 ? launch_int8<BigI8, true>(a, s) : launch_int8<BigI8, false>(a, s);
   return bf16 ? launch_int8<MidI8, true>(a, s) : launch_int8<MidI8, false>(a, s);
 }

@@ -423,6 +423,37 @@ __device__ __forceinline__ void tile_of_block(uint32_t bid, uint32_t n_wg, uint3
   tn = __builtin_amdgcn_readfirstlane((int)c);
 }
 
+// 256 x 256 tiles (one workgroup a CU) or 128 x 128 (two)?  And, for a product whose
+// k may be split with the parts joined afterwards, over how many workgroups?  The
+// fewer rounds of the chip: a CU's two small tiles take 0.58 of a large one's time
+// (1140 against 1330 TFLOP/s), and no share is shorter than eight steps.
+struct TilePlan {
+  bool big;
+  int splits;
+};
+inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, bool may_split, int cus) {
+  TilePlan best{false, 1};
+  double least = 0;
+  for (int big = 0; big < 2; ++big) {
+    const int64_t b = big ? 256 : 128, slots = big ? cus : 2ll * cus;
+    const int64_t tiles = ((m + b - 1) / b) * ((n + b - 1) / b);
+    int64_t s = 1;
+    if (may_split) {
+      s = slots / (tiles > 0 ? tiles : 1);
+      s = s > steps / 8 ? steps / 8 : s;
+      s = s < 1 ? 1 : s > 64 ? 64 : s;
+    }
+    const double rounds = (double)((tiles * s + slots - 1) / slots);
+    // (eight steps' time for a tile's start and end)
+    const double t = rounds * (big ? 1.0 : 0.58) * (double)((steps + s - 1) / s + 8);
+    if (big == 0 || t < least) {
+      least = t;
+      best = TilePlan{big != 0, (int)s};
+    }
+  }
+  return best;
+}
+
 // row of a 32 x 32 accumulator block held in register r of lane half h
 __device__ __forceinline__ constexpr int acc_row(int r, int h) {
   return (r & 3) + 8 * (r >> 2) + 4 * h;

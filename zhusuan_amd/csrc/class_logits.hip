@@ -595,12 +595,15 @@ struct ClassLayout {
   bool whole;                      // float32 operands as they are, no planes
   int64_t piece, pieces;           // gradient: classes per piece
   int64_t resid_pitch, resid_plane;
-  int64_t resid, dx_part, bias_part;
-  int dx_splits, dx_tile, dw_tile;
+  int64_t resid, bias_part;
+  int64_t dx_part, dw_part;        // float32 parts, where there is more than one
+  int dx_splits, dx_tile, dw_splits, dw_tile;
   int64_t total;
 };
 
 int64_t tiles(int64_t n, int64_t b) { return (n + b - 1) / b; }
+
+int clip(int splits, int64_t steps) { return (int)(splits < steps ? splits : steps); }
 
 ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   ClassLayout l;
@@ -637,10 +640,13 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
            : plan_tiles(l.piece, q.n, terms * tiles(q.d * element, 128), false, cus).big ? 0
                                                                                          : 1;
   // (half the chip or more without a tile: halve them.  float32 1065 x 3456, 1122
-  // classes: 81 tiles 84 us, 153 halves 73)
-  if (l.tile == 1 && tiles(l.piece, 128) * tiles(q.n, 128) * 2 <= cus) l.tile = 2;
+  // classes: 81 tiles 84 us, 153 halves 73; 128 x 2048, 4096 classes: 64 halves 82 us,
+  // 128 quarters 50)
+  while (l.tile > 0 && l.tile < 3 &&
+         tiles(l.piece, 128) * tiles(q.n, kTileRows[l.tile]) * 2 <= cus)
+    ++l.tile;
   l.tiles_v = tiles(q.v, kTileClasses[l.tile]);
-  l.part = l.label_logit = l.resid = l.dx_part = l.bias_part = 0;
+  l.part = l.label_logit = l.resid = l.dx_part = l.dw_part = l.bias_part = 0;
   if (!grad) {
     l.part = take(l.tiles_v * q.n * 8);
     l.label_logit = take(q.n * 4);
@@ -648,13 +654,14 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     l.resid_pitch = round_up(l.piece * (l.whole ? 4 : 2), 128);
     l.resid_plane = q.n * l.resid_pitch;
     l.resid = take(l.planes * l.resid_plane);
-    l.dw_tile = plan_tiles(l.piece, q.d, terms * tiles(q.n * element, 128), false, cus).big ? 0
-                                                                                            : 1;
+    const TilePlan dw = plan_tiles(l.piece, q.d, terms * tiles(q.n * element, 128), true, cus);
+    l.dw_tile = dw.big ? 0 : 1;
+    l.dw_splits = clip(dw.splits, tiles(q.n * element, 128));
+    if (l.dw_splits > 1) l.dw_part = take(l.dw_splits * l.piece * q.d * 4);
     const TilePlan dx = plan_tiles(q.n, q.d, terms * tiles(l.piece * element, 128), true, cus);
     l.dx_tile = q.n <= 32 ? 3 : q.n <= 64 ? 2 : dx.big ? 0 : 1;
-    const int64_t steps = tiles(l.piece * element, 128);
-    l.dx_splits = (int)(dx.splits < steps ? dx.splits : steps);
-    l.dx_part = take(l.dx_splits * q.n * q.d * 4);
+    l.dx_splits = clip(dx.splits, tiles(l.piece * element, 128));
+    if (l.dx_splits * l.pieces > 1) l.dx_part = take(l.dx_splits * q.n * q.d * 4);
     l.bias_part = take(tiles(q.n, kTileRows[l.tile]) * q.v * 4);
   }
   l.total = at;
@@ -716,6 +723,18 @@ int launch_gradient(const ClassArgs& g, const ClassLayout& l, int tile, hipStrea
   return l.planes > 1 ? launch_gradient_of<BK, MmaF16, 2>(g, tile, s)
          : l.whole    ? launch_gradient_of<BK, MmaF32, 1>(g, tile, s)
                       : launch_gradient_of<BK, MmaBf16, 0>(g, tile, s);
+}
+
+int sum_rows(const void* parts, int n_parts, int64_t n, bool f32, void* out, hipStream_t s) {
+  const float* x = static_cast<const float*>(parts);
+  if (f32)
+    hipLaunchKernelGGL(sum_rows_kernel<false>, dim3(grid_for(n)), dim3(256), 0, s, x, n_parts, n,
+                       n, out);
+  else
+    hipLaunchKernelGGL(sum_rows_kernel<true>, dim3(grid_for(n)), dim3(256), 0, s, x, n_parts, n,
+                       n, out);
+  ZS_LAUNCH_CHECK("sum_rows_kernel launch");
+  return ZSHMC_OK;
 }
 
 // The operands X and w, packed where they have to be; `labels`: rows of X that are
@@ -894,6 +913,7 @@ extern "C" int zshmc_class_log_prob_grad(
   const int terms = l.planes > 1 ? kTermsSplit : 1;
   const int64_t pb = l.whole ? 4 : 2;            // bytes of a plane's element
   const float* scales = reinterpret_cast<const float*>(ws + l.scales);
+  const bool dx_joined = l.dx_splits * l.pieces > 1;
   for (int64_t c0 = 0; c0 < q.v; c0 += l.piece) {
     const int64_t c = q.v - c0 < l.piece ? q.v - c0 : l.piece;
     TileOperand wp = ow;
@@ -937,11 +957,19 @@ extern "C" int zshmc_class_log_prob_grad(
       g.terms = terms;
       g.scale_m = scales;
       g.scale_n = scales + 2;
-      g.splits = 1;
-      g.out = static_cast<unsigned char*>(grad_w) + c0 * q.d * q.esize();
+      g.splits = l.dw_splits;
       g.out_ld = q.d;
-      g.out_bf16 = !q.f32();
+      void* const dw = static_cast<unsigned char*>(grad_w) + c0 * q.d * q.esize();
+      if (l.dw_splits > 1) {
+        g.out = ws + l.dw_part;
+        g.out_split = c * q.d;
+      } else {
+        g.out = dw;
+        g.out_bf16 = !q.f32();
+      }
       rc = launch_gradient<true>(g, l, l.dw_tile, s);
+      if (rc != ZSHMC_OK) return rc;
+      if (l.dw_splits > 1) rc = sum_rows(g.out, l.dw_splits, c * q.d, q.f32(), dw, s);
       if (rc != ZSHMC_OK) return rc;
     }
     if (grad_x) {                  // dX += r w over the piece's classes
@@ -956,30 +984,24 @@ extern "C" int zshmc_class_log_prob_grad(
       g.g = grad_log_prob;
       g.row_units = 1;
       g.splits = l.dx_splits;
-      g.out = ws + l.dx_part;
       g.out_ld = q.d;
-      g.out_split = q.n * q.d;
-      g.accumulate = c0 > 0;
+      if (dx_joined) {
+        g.out = ws + l.dx_part;
+        g.out_split = q.n * q.d;
+        g.accumulate = c0 > 0;
+      } else {
+        g.out = grad_x;
+        g.out_bf16 = !q.f32();
+      }
       rc = launch_gradient<false>(g, l, l.dx_tile, s);
       if (rc != ZSHMC_OK) return rc;
     }
   }
-  if (grad_x) {
-    const float* parts = reinterpret_cast<const float*>(ws + l.dx_part);
-    const int64_t n = q.n * q.d;
-    if (q.f32())
-      hipLaunchKernelGGL(sum_rows_kernel<false>, dim3(grid_for(n)), dim3(256), 0, s, parts,
-                         l.dx_splits, n, n, grad_x);
-    else
-      hipLaunchKernelGGL(sum_rows_kernel<true>, dim3(grid_for(n)), dim3(256), 0, s, parts,
-                         l.dx_splits, n, n, grad_x);
-    ZS_LAUNCH_CHECK("sum_rows_kernel launch");
+  if (grad_x && dx_joined) {
+    rc = sum_rows(ws + l.dx_part, l.dx_splits, q.n * q.d, q.f32(), grad_x, s);
+    if (rc != ZSHMC_OK) return rc;
   }
-  if (grad_bias) {
-    hipLaunchKernelGGL(sum_rows_kernel<false>, dim3(grid_for(q.v)), dim3(256), 0, s,
-                       reinterpret_cast<const float*>(ws + l.bias_part),
-                       (int)tiles(q.n, kTileRows[l.tile]), q.v, q.v, grad_bias);
-    ZS_LAUNCH_CHECK("sum_rows_kernel launch");
-  }
-  return ZSHMC_OK;
+  if (grad_bias)
+    rc = sum_rows(ws + l.bias_part, (int)tiles(q.n, kTileRows[l.tile]), q.v, true, grad_bias, s);
+  return rc;
 }

@@ -424,9 +424,11 @@ __device__ __forceinline__ void tile_of_block(uint32_t bid, uint32_t n_wg, uint3
 }
 
 // 256 x 256 tiles (one workgroup a CU) or 128 x 128 (two)?  And, for a product whose
-// k may be split with the parts joined afterwards, over how many workgroups?  The
-// fewer rounds of the chip: a CU's two small tiles take 0.58 of a large one's time
-// (1140 against 1330 TFLOP/s), and no share is shorter than eight steps.
+// k may be split with the parts joined afterwards, over how many workgroups?  What
+// takes the fewest of a large tile's steps (0.9 us): a CU's two small tiles take 0.58
+// of a large one's time (1140 against 1330 TFLOP/s); a tile's start and end cost eight
+// steps, and no share is shorter than that; parts are written and read by a launch of
+// their own.
 struct TilePlan {
   bool big;
   int splits;
@@ -437,18 +439,20 @@ inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, bool may_split, 
   for (int big = 0; big < 2; ++big) {
     const int64_t b = big ? 256 : 128, slots = big ? cus : 2ll * cus;
     const int64_t tiles = ((m + b - 1) / b) * ((n + b - 1) / b);
-    int64_t s = 1;
+    int64_t most = 1;
     if (may_split) {
-      s = slots / (tiles > 0 ? tiles : 1);
-      s = s > steps / 8 ? steps / 8 : s;
-      s = s < 1 ? 1 : s > 64 ? 64 : s;
+      most = slots / (tiles > 0 ? tiles : 1);
+      most = most > steps / 8 ? steps / 8 : most;
+      most = most < 1 ? 1 : most > 64 ? 64 : most;
     }
-    const double rounds = (double)((tiles * s + slots - 1) / slots);
-    // (eight steps' time for a tile's start and end)
-    const double t = rounds * (big ? 1.0 : 0.58) * (double)((steps + s - 1) / s + 8);
-    if (big == 0 || t < least) {
-      least = t;
-      best = TilePlan{big != 0, (int)s};
+    for (int64_t s = 1; s <= most; s = s < most && 2 * s > most ? most : 2 * s) {
+      const double rounds = (double)((tiles * s + slots - 1) / slots);
+      const double t = rounds * (big ? 1.0 : 0.58) * (double)((steps + s - 1) / s + 8) +
+                       (s > 1 ? 5.0 + 2e-6 * (double)(m * n * s) : 0.0);
+      if ((big == 0 && s == 1) || t < least) {
+        least = t;
+        best = TilePlan{big != 0, (int)s};
+      }
     }
   }
   return best;

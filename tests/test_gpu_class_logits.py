@@ -91,6 +91,23 @@ def test_rows_of_different_sizes():
         check(w, X, y, b, g)
 
 
+def test_a_row_far_larger_than_the_others():
+    """One row of 1e25: the others' log-probabilities, and their rows of dX,
+    are what they are without it."""
+    w, X, y, b, g = problem(300, 96, 700, torch.float32, 57, bias=True)
+    X2 = X.clone()
+    X2[7] *= 1e25
+    others = torch.arange(300, device='cuda') != 7
+    got = []
+    for x in (X, X2):
+        x = x.clone().requires_grad_()
+        lp = zs.linear_categorical_log_prob(w, x, y, bias=b)
+        got.append((lp.detach()[others],
+                    torch.autograd.grad(lp, x, g)[0][others]))
+    assert torch.equal(got[0][0], got[1][0])
+    assert torch.equal(got[0][1], got[1][1])
+
+
 @pytest.mark.parametrize('dtype', BOTH)
 def test_every_row_ignored(dtype):
     w, X, y, b, g = problem(20, 64, 100, dtype, 6, True)

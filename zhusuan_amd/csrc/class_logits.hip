@@ -55,14 +55,17 @@ __device__ __forceinline__ float near_2_14(float x) {
   return __builtin_bit_cast(float, (uint32_t)(e - 13 + 127) << 23);
 }
 
-// Rows to be packed, and the largest finite magnitudes of X, w and g that their
-// scales come from, per workgroup, without the rows (of X and g) that are ignored.
+// Rows to be packed, and the largest finite magnitudes that their scales come from:
+// of each row of X (a row's logits are as good as its own values allow, whatever the
+// other rows hold), and of X, w and g per workgroup, without the rows (of X and g)
+// that are ignored.
 constexpr int kMaxParts = 1024;
 struct PackJob {
   const void* src;
   int64_t rows, cols, ld;
   unsigned char* dst;
   const int64_t* labels;           // rows labelled `ignore` become zeros; or NULL
+  const float* row_max;            // rows have a scale each: or NULL
   const float* row_g;              // rows are scaled like g's: or NULL
   int part, part_g;                // whose maximum
   int writes;                      // the first workgroup writes scale[part] ( + [part_g])
@@ -72,6 +75,7 @@ struct PackArgs {
   int64_t pitch, ignore;
   const float* part;               // [3][kMaxParts]
   float* scale;                    // [3]
+  float* row_max;                  // [rows of X]
 };
 
 __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* __restrict__ g,
@@ -87,10 +91,7 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
     v = fabsf(v);
     mx = v <= 3.402823466e38f ? fmaxf(mx, v) : mx;
   };
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / groups, c = (i - r * groups) * 4;
-    if (j.labels && j.labels[r] == a.ignore) continue;
+  auto four = [&](int64_t r, int64_t c) {
     const float* from = src + r * ld + c;
     if (c + 4 <= cols) {
       typedef float any __attribute__((ext_vector_type(4), aligned(4)));
@@ -99,6 +100,27 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
       for (int e = 0; e < 4; ++e) widen(v[e]);
     } else {
       for (int e = 0; e < cols - c; ++e) widen(from[e]);
+    }
+  };
+  if (k == 0) {                    // a wave a row
+    float all = 0.f;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows;
+         r += (int64_t)gridDim.x * 4) {
+      mx = 0.f;
+      if (!(j.labels && j.labels[r] == a.ignore))
+        for (int64_t c = (threadIdx.x & 63) * 4; c < cols; c += 256) four(r, c);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+      if ((threadIdx.x & 63) == 0) a.row_max[r] = mx;
+      all = fmaxf(all, mx);
+    }
+    mx = all;
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * 256) {
+      const int64_t r = i / groups;
+      if (j.labels && j.labels[r] == a.ignore) continue;
+      four(r, (i - r * groups) * 4);
     }
   }
 #pragma unroll
@@ -112,7 +134,7 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
 
 // blockIdx.y's rows of `cols` elements -> rows of `pitch` bytes, zero behind the
 // last column: elements as they are, or (SPLIT) float32 as two float16 planes of x /
-// scale.  Rows whose label is `ignore` become zeros (whatever they hold, NaN
+// scale, the row's or all rows'.  Rows whose label is `ignore` become zeros (whatever they hold, NaN
 // included, reaches no product).
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
@@ -166,11 +188,13 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
     unsigned char* const to = j.dst + r * a.pitch + (i - r * groups) * 16;
     if constexpr (SPLIT) {
       // (powers of two: the products are exact)
-      const float f = j.row_g ? inv_g * near_2_14(j.row_g[r]) : 1.f;
+      const float f = j.row_max ? 1.f / near_2_14(j.row_max[r])
+                      : j.row_g ? inv_g * near_2_14(j.row_g[r]) : 1.f;
+      const float one = j.row_max ? 1.f : inv;
       tu4 hi, lo;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float x = v[2 * q] * inv * f, y = v[2 * q + 1] * inv * f;
+        const float x = v[2 * q] * one * f, y = v[2 * q + 1] * one * f;
         hi[q] = f16_pair(x, y);
         lo[q] = f16_pair(f16_rest(x), f16_rest(y));
       }
@@ -220,9 +244,9 @@ struct ClassArgs {
   int64_t out_ld, out_split;       // elements; split s at out + s * out_split
   int out_bf16, accumulate;
   // float32 as planes: what the accumulators count in is *scale_m * *scale_n of
-  // the operands' units; a row of r is in units of its own, near_2_14(g), which a
-  // product over the classes has in place of *scale_n (row_units)
-  const float *scale_m, *scale_n;
+  // the operands' units; in place of *scale_n a row of X has near_2_14(row_x[n]), and
+  // a row of r, in a product over the classes (row_units), near_2_14(g[n])
+  const float *scale_m, *scale_n, *row_x;
   int row_units;
 };
 
@@ -303,16 +327,21 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
   }
 
   // what an accumulator counts in: planes of scaled operands
-  float unit_m = 1.f, unit_n = 1.f;
-  float unit_r[C::WN];
+  float unit_m = 1.f;
+  float unit_n[C::WN], unit_r[C::WN];
   if (F32 == 2) {
     unit_m = *p.scale_m;
-    if (EPI != kEpiStore || !p.row_units) unit_n = *p.scale_n;
-    if (EPI != kEpiStats) {
+    const bool rows = EPI == kEpiStore && !p.row_units;
 #pragma unroll
-      for (int j = 0; j < C::WN; ++j) {
-        const int64_t n = n0 + nw + j * 32 + col;
-        unit_r[j] = (EPI == kEpiResidual || p.row_units) && n < p.n ? near_2_14(p.g[n]) : 1.f;
+    for (int j = 0; j < C::WN; ++j) {
+      const int64_t n = n0 + nw + j * 32 + col;
+      unit_n[j] = unit_r[j] = 1.f;
+      if (rows)
+        unit_n[j] = *p.scale_n;
+      else if (n < p.n) {
+        if (EPI != kEpiStore) unit_n[j] = near_2_14(p.row_x[n]);
+        if (EPI == kEpiStore) unit_n[j] = near_2_14(p.g[n]);
+        if (EPI == kEpiResidual) unit_r[j] = near_2_14(p.g[n]);
       }
     }
   }
@@ -321,7 +350,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         v[r] = acc_get(acc[decltype(I)::value][decltype(J)::value], 4 * decltype(Q)::value + r);
-        if (F32 == 2) v[r] = v[r] * unit_m * unit_n * unit_r[decltype(J)::value];
+        if (F32 == 2) v[r] = v[r] * unit_m * unit_n[decltype(J)::value];
       }
     };
     if (F32 == 0 && p.out_bf16) {
@@ -368,7 +397,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         l[r] = acc_get(acc[i][j], 4 * q + r);
-        if (F32 == 2) l[r] = l[r] * unit_m * unit_n;
+        if (F32 == 2) l[r] = l[r] * unit_m * unit_n[j];
         if (decltype(BIASED)::value) l[r] += bias[i][q][r];
       }
     };
@@ -588,7 +617,7 @@ struct ClassLayout {
   int64_t x_plane, w_plane, planes;
   bool pack_x, pack_w;
   int64_t xp, wp, xg;              // offsets; xg: X with its rows scaled like g's
-  int64_t maxima, scales;          // float32 in planes: of X, w, g
+  int64_t maxima, scales, row_max; // float32 in planes: of X, w, g; of X's rows
   int64_t part, label_logit;       // forward
   int tile;                        // see kTileClasses
   int64_t tiles_v;                 // parts of the statistics
@@ -623,6 +652,7 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   };
   l.maxima = l.planes > 1 ? take(3ll * kMaxParts * 4) : 0;
   l.scales = l.planes > 1 ? take(3 * 4) : 0;
+  l.row_max = l.planes > 1 ? take(q.n * 4) : 0;
   l.xp = l.pack_x ? take(l.planes * l.x_plane) : 0;
   l.wp = l.pack_w ? take(l.planes * l.w_plane) : 0;
   l.xg = grad && l.planes > 1 ? take(l.planes * l.x_plane) : 0;
@@ -747,10 +777,13 @@ int operands(const ClassProblem& q, const ClassLayout& l, unsigned char* ws,
   const int64_t e = q.esize();
   *x = TileOperand{static_cast<const unsigned char*>(q.x), q.ldx * e, 0, q.n, q.d * e};
   *w = TileOperand{static_cast<const unsigned char*>(q.w), q.ldw * e, 0, q.v, q.d * e};
-  const PackJob jx{q.x, q.n, q.d, q.ldx, ws + l.xp, labels, nullptr, 0, g ? 2 : 0, 1};
-  const PackJob jw{q.w, q.v, q.d, q.ldw, ws + l.wp, nullptr, nullptr, 1, 1, 1};
+  const PackJob jx{q.x, q.n, q.d, q.ldx, ws + l.xp, labels,
+                   l.planes > 1 ? reinterpret_cast<const float*>(ws + l.row_max) : nullptr,
+                   nullptr, 0, g ? 2 : 0, 1};
+  const PackJob jw{q.w, q.v, q.d, q.ldw, ws + l.wp, nullptr, nullptr, nullptr, 1, 1, 1};
   PackJob jg = jx;
   jg.dst = ws + l.xg;
+  jg.row_max = nullptr;
   jg.row_g = g;
   jg.part_g = 2;
   jg.writes = 0;
@@ -761,6 +794,7 @@ int operands(const ClassProblem& q, const ClassLayout& l, unsigned char* ws,
   a.ignore = ignore;
   a.part = reinterpret_cast<const float*>(ws + l.maxima);
   a.scale = reinterpret_cast<float*>(ws + l.scales);
+  a.row_max = reinterpret_cast<float*>(ws + l.row_max);
   int jobs = 0;
   int64_t most = 0;
   auto add = [&](const PackJob& j) {
@@ -864,8 +898,8 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   a.n = q.n;
   a.steps = (int)tiles(q.d * (l.whole ? 4 : 2), 128);
   a.terms = l.planes > 1 ? kTermsSplit : 1;
-  a.scale_n = reinterpret_cast<const float*>(ws + l.scales);
-  a.scale_m = a.scale_n + 1;
+  a.scale_m = reinterpret_cast<const float*>(ws + l.scales) + 1;
+  a.row_x = reinterpret_cast<const float*>(ws + l.row_max);
   a.splits = 1;
   a.bias = bias;
   a.labels = labels;
@@ -927,8 +961,8 @@ extern "C" int zshmc_class_log_prob_grad(
     a.n = q.n;
     a.steps = (int)tiles(q.d * pb, 128);
     a.terms = terms;
-    a.scale_n = scales;
     a.scale_m = scales + 1;
+    a.row_x = reinterpret_cast<const float*>(ws + l.row_max);
     a.splits = 1;
     a.bias = bias ? bias + c0 : nullptr;
     a.labels = labels;

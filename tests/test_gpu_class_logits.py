@@ -1,10 +1,12 @@
 """zs.linear_categorical_log_prob (csrc/class_logits.hip) against its plain
 form in 64 bits, with the element-wise bounds of helpers_class_logits."""
+import math
+
 import pytest
 import torch
 
 import zhusuan_amd as zs
-from helpers_class_logits import class_log_prob, problem, within
+from helpers_class_logits import U32, class_log_prob, problem, within
 
 pytestmark = pytest.mark.gpu
 BOTH = [torch.float32, torch.bfloat16]
@@ -306,3 +308,87 @@ def test_captured_and_replayed(dtype):
         for a, c in zip(out, step()):
             assert torch.equal(a, c)
         torch.randn(1000, 1000, device='cuda').sum().item()
+
+
+def test_categorical_over_many_classes_takes_them_in_pieces():
+    """Categorical(linear_class_logits(w, X)) of two chains: log_prob and its
+    gradients, without the [2, N, V] logits."""
+    N, D, V = 3000, 40, 1500
+    cases = [problem(N, D, V, torch.float32, 30 + c) for c in range(2)]
+    X = cases[0][1].requires_grad_()
+    y = cases[0][2]
+    w = torch.stack([c[0] for c in cases]).requires_grad_()
+    for labels in (y.to(torch.int32), y.float(), y[None],
+                   torch.stack([y, y])):
+        dist = zs.distributions.Categorical(zs.linear_class_logits(w, X),
+                                            group_ndims=1)
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        lp = dist.log_prob(labels)
+        assert lp.shape == (2,)
+        gw, gx = torch.autograd.grad(lp.sum(), (w, X))
+        assert dist._logits_dense is None
+        assert torch.cuda.max_memory_allocated() - before < 2 * N * V * 4
+        tol_x = ref_x = 0
+        for c in range(2):
+            # (w's gradient: row by row, as if the other chain were not there)
+            (lp64, (dw, dx, _)), (tol, (tw, tx, _)) = class_log_prob(
+                w[c], X, y, g=torch.ones(N, device='cuda'))
+            # N rows' sum in float32, in any order
+            within(lp[c], lp64.sum(), tol.sum() + N * U32 * lp64.abs().sum())
+            within(gw[c], dw, tw)
+            ref_x, tol_x = ref_x + dx, tol_x + tx + U32 * dx.abs()
+        within(gx, ref_x, tol_x + U32 * ref_x.abs())
+    # labels of a shape of their own: the logits are written out
+    dist = zs.distributions.Categorical(zs.linear_class_logits(w, X))
+    with torch.no_grad():
+        lp3 = dist.log_prob(y.expand(3, 1, N))
+        one = zs.linear_categorical_log_prob(w[1], X, y)
+    assert lp3.shape == (3, 2, N)
+    # (float32 sums of D terms either way, and two log-sum-exps)
+    lp64, tol = class_log_prob(w[1], X, y)
+    within(lp3[2, 1], lp64, 2 * tol)
+    within(one, lp64, tol)
+    with pytest.raises(ValueError):
+        dist.log_prob(y[:-1])
+
+
+def test_sampler_of_a_softmax_regression_over_many_classes():
+    """A model with a [V, D] latent a chain, its logits spelled X @ w^T:
+    log_joint and its gradient, and transitions of the sampler."""
+    N, D, V, C = 2100, 24, 2048, 2
+    w0, X, y, _, _ = problem(N, D, V, torch.float32, 41)
+    w1 = problem(N, D, V, torch.float32, 42)[0]
+
+    @zs.meta_bayesian_net()
+    def model():
+        bn = zs.BayesianNet()
+        w = bn.normal('w', torch.zeros(V, D, device='cuda'), std=1.,
+                      n_samples=C, group_ndims=2)
+        bn.categorical('y', X.unsqueeze(0) @ w.tensor.transpose(-1, -2),
+                       group_ndims=1)
+        return bn
+
+    labels = y.to(torch.int32)
+    leaf = torch.stack([w0, w1]).requires_grad_()
+    lj = model().observe(w=leaf, y=labels).log_joint()
+    assert lj.shape == (C,)
+    got, = torch.autograd.grad(lj.sum(), leaf)
+    for c in range(C):
+        wc = leaf[c].detach()
+        (lp, (dw, _, _)), (tol, (tw, _, _)) = class_log_prob(
+            wc, X, y, g=torch.ones(N, device='cuda'))
+        within(got[c], dw - wc.double(),
+               tw + 4 * U32 * (dw.abs() + wc.abs()))
+        prior = -0.5 * wc.double().square() - 0.5 * math.log(2 * math.pi)
+        within(lj[c], lp.sum() + prior.sum(), tol.sum() + U32 * (
+            N * lp.abs().sum() + (V * D + 8) * prior.abs().sum()))
+
+    q = torch.zeros(C, V, D, device='cuda')
+    hmc = zs.HMC(step_size=1e-3, n_leapfrogs=2)
+    op, info = hmc.sample(model(), {'y': labels}, {'w': q})
+    assert hmc.plan_kind == 'generic'
+    for _ in range(3):
+        op.run()
+    assert bool(torch.isfinite(info.log_prob).all())
+    assert bool(q.isfinite().all()) and float(q.abs().max()) > 0

@@ -455,7 +455,15 @@ class LinearClassLogits(object):
     `Categorical(linear_class_logits(w, X), group_ndims=1)` evaluates log_prob
     and its gradient with the fused fp32-MFMA kernels
     (zshmc_linear_categorical_log_lik; up to 32 classes x 1024 features);
-    anything else falls back to `.dense()`."""
+    log_prob of many classes takes them in pieces, chain by chain
+    (`linear_categorical_log_prob`); anything else falls back to `.dense()`."""
+
+    # From how many logits a chain, and classes, log_prob takes the classes in
+    # pieces rather than writing the logits out: float32, 1024 x 784, log_prob
+    # with its gradient over 4096 classes (2^22) 146 us against 221, over 512
+    # (2^19) 145 against 178 of a host's time either way; 8192 x 2048 over 512
+    # classes 340 against 267, over 4096 1270 against 2010.
+    MANY_LOGITS, MANY_CLASSES = 1 << 22, 1024
 
     def __init__(self, w, X):
         w = as_tensor(w)          # (a symbolic latent: the latent itself)
@@ -498,6 +506,25 @@ class LinearClassLogits(object):
         return (self.n_classes <= _ops.MAX_CLASSES and
                 self.n_features <= _ops.MAX_LIKELIHOOD_WIDTH and
                 not self.X.requires_grad and self.dtype == torch.float32)
+
+    def many_ok(self):
+        return (self.n_classes >= self.MANY_CLASSES and
+                self.n_rows * self.n_classes >= self.MANY_LOGITS and
+                self.dtype == torch.float32 and
+                self.X.dtype == torch.float32 and
+                self.w.device == self.X.device and self.w.is_cuda)
+
+    def log_prob(self, labels):
+        """log Categorical of `labels` [lead..., N], a chain's classes at a
+        time in pieces: [lead..., N]."""
+        lead = self.lead_shape
+        if not lead:
+            return _ops.linear_categorical_log_prob(self.w, self.X, labels)
+        w = self.w.reshape((-1,) + tuple(self.w.shape[-2:]))
+        y = labels.reshape(-1, self.n_rows)
+        rows = [_ops.linear_categorical_log_prob(w_c, self.X, y_c)
+                for w_c, y_c in zip(w.unbind(0), y.unbind(0))]
+        return torch.stack(rows).reshape(lead + (self.n_rows,))
 
     def dense(self):
         return torch.matmul(self.X, self.w.transpose(-1, -2))
@@ -612,13 +639,17 @@ class Categorical(Distribution):
 
     def _log_prob(self, given):
         # :499-505 explicit broadcast of given vs logits[..., :-1]
+        shape = self._lazy.shape if self._lazy is not None \
+            else self._logits.shape
         try:
-            batch = broadcast_shapes(given.shape,
-                                           self._logits.shape[:-1])
+            batch = broadcast_shapes(given.shape, shape[:-1])
         except RuntimeError:
             raise ValueError(
                 "given and logits cannot broadcast to match. ({} vs. {})"
-                .format(tuple(given.shape), tuple(self._logits.shape)))
+                .format(tuple(given.shape), tuple(shape)))
+        if self._lazy is not None and self._logits_dense is None and \
+                tuple(batch) == tuple(shape[:-1]) and self._lazy.many_ok():
+            return self._lazy.log_prob(given.expand(batch).to(torch.int64))
         labels = given.expand(batch).to(torch.int64).contiguous().reshape(-1)
         logits = self._logits.expand(tuple(batch) + (self._n_categories,)) \
             .contiguous().reshape(-1, self._n_categories)

@@ -232,3 +232,41 @@ def test_an_output_layer_trained_rounded_and_used():
         lp = d.log_prob(y)
         ref = torch.log_softmax(logits.double(), 1).gather(1, y[:, None])[:, 0]
         within(lp, ref, 64 * 2.0 ** -24 * (1 + logits.abs().double().amax(1)))
+
+
+def test_no_gradient_is_refused():
+    w = zs.quantize_rows(torch.randn(20, 16, device='cuda'))
+    X = torch.randn(3, 16, device='cuda')
+    b = torch.randn(20, device='cuda')
+    ref = zs.quantized_linear(w, X, bias=b)
+    for kw in (dict(X=X.clone().requires_grad_()),
+               dict(bias=b.clone().requires_grad_())):
+        kw = dict(dict(X=X, bias=b), **kw)
+        with pytest.raises(RuntimeError, match='gradient'):
+            zs.quantized_linear(w, **kw)
+        with torch.no_grad():
+            assert torch.equal(zs.quantized_linear(w, **kw), ref)
+
+
+def test_a_categorical_answers_from_8_bit_rows():
+    """Categorical(linear_class_logits(quantize_rows(w), X)): its logits are
+    quantized_linear's, and labels are scored and drawn from them."""
+    gen = torch.Generator().manual_seed(3)
+    w = torch.randn(300, 96, generator=gen).cuda()
+    X = torch.randn(40, 96, generator=gen).cuda()
+    y = torch.randint(300, (40,), generator=gen, dtype=torch.int32).cuda()
+    q = zs.quantize_rows(w)
+    dist = zs.distributions.Categorical(zs.linear_class_logits(q, X),
+                                        group_ndims=1)
+    logits = zs.quantized_linear(q, X)
+    assert dist.get_batch_shape() == (40,)
+    assert torch.equal(dist.logits, logits)
+    plain = zs.distributions.Categorical(logits, group_ndims=1)
+    assert torch.equal(dist.log_prob(y), plain.log_prob(y))
+    drawn = dist.sample(7)
+    assert drawn.shape == (7, 40)
+    assert int(drawn.min()) >= 0 and int(drawn.max()) < 300
+    with pytest.raises(ValueError):
+        zs.linear_class_logits(q, X[:, :95])
+    with pytest.raises(ValueError):
+        zs.linear_class_logits(zs.quantize_rows(w.reshape(2, 150, 96)), X)

@@ -1294,7 +1294,8 @@ def quantized_linear(w, X, bias=None, dtype=None):
     scale per output channel), X [..., K] a float32 / bfloat16 tensor -- rounded
     to 8 bits per row here -- or a `QuantizedRows`.  The integer sum is exact;
     out[..., v] = (scale_x scale_w[v]) * sum + bias[v] in float32, rounded once to
-    `dtype` (X's own, float32 for a QuantizedRows).  K <= 131072.  No gradient."""
+    `dtype` (X's own, float32 for a QuantizedRows).  K <= 131072.  No gradient:
+    an X or bias that requires one is refused while gradients are recorded."""
     if not isinstance(w, QuantizedRows) or len(w._shape) != 2:
         raise TypeError("quantized_linear: w must be QuantizedRows [V, K]")
     X = _symbolic.force(X.tensor if hasattr(X, 'tensor') else X)
@@ -1320,9 +1321,15 @@ def quantized_linear(w, X, bias=None, dtype=None):
             raise ValueError("quantized_linear: bias must be a float tensor "
                              "[{}]".format(V))
         require_device(bias)
-        bias = _float_row(bias)
+        if bias.dtype != _F32 or not bias.is_contiguous():
+            bias = bias.to(_F32).contiguous()
     if X.device != w.device or (bias is not None and bias.device != w.device):
         raise ValueError("quantized_linear: all tensors must be on one device")
+    if torch.is_grad_enabled() and any(
+            isinstance(t, torch.Tensor) and t.requires_grad
+            for t in (X, bias)):
+        raise RuntimeError("quantized_linear: has no gradient; detach X and "
+                           "bias, or call it under torch.no_grad()")
     out = torch.empty(X.shape[:-1] + (V,), dtype=dtype, device=w.device)
     if not out.numel():
         return out

@@ -456,7 +456,9 @@ class LinearClassLogits(object):
     and its gradient with the fused fp32-MFMA kernels
     (zshmc_linear_categorical_log_lik; up to 32 classes x 1024 features);
     log_prob of many classes takes them in pieces, chain by chain
-    (`linear_categorical_log_prob`); anything else falls back to `.dense()`."""
+    (`linear_categorical_log_prob`); anything else falls back to `.dense()`.
+    w may also be the 8-bit rows [K, F] that `quantize_rows` returns: a model
+    that is done learning answers from them (`quantized_linear`, no gradient)."""
 
     # From how many logits a chain, and classes, log_prob takes the classes in
     # pieces rather than writing the logits out: float32, 1024 x 784, log_prob
@@ -466,9 +468,11 @@ class LinearClassLogits(object):
     MANY_LOGITS, MANY_CLASSES = 1 << 22, 1024
 
     def __init__(self, w, X):
-        w = as_tensor(w)          # (a symbolic latent: the latent itself)
+        if not isinstance(w, _ops.QuantizedRows):
+            w = as_tensor(w)      # (a symbolic latent: the latent itself)
         X = as_tensor(X)
-        if X.dim() != 2 or w.dim() < 2 or w.shape[-1] != X.shape[-1]:
+        if X.dim() != 2 or len(w.shape) < 2 or w.shape[-1] != X.shape[-1] or (
+                isinstance(w, _ops.QuantizedRows) and len(w.shape) != 2):
             raise ValueError(
                 "linear_class_logits: w[..., K, F] and X[N, F] expected, got "
                 "{} and {}".format(tuple(w.shape), tuple(X.shape)))
@@ -495,20 +499,25 @@ class LinearClassLogits(object):
         return torch.Size(self.lead_shape + (self.n_rows, self.n_classes))
 
     @property
+    def quantized(self):
+        return isinstance(self.w, _ops.QuantizedRows)
+
+    @property
     def dtype(self):
-        return self.w.dtype
+        return torch.float32 if self.quantized else self.w.dtype
 
     @property
     def device(self):
         return self.w.device
 
     def fused_ok(self):
-        return (self.n_classes <= _ops.MAX_CLASSES and
+        return (not self.quantized and self.n_classes <= _ops.MAX_CLASSES and
                 self.n_features <= _ops.MAX_LIKELIHOOD_WIDTH and
                 not self.X.requires_grad and self.dtype == torch.float32)
 
     def many_ok(self):
-        return (self.n_classes >= self.MANY_CLASSES and
+        return (not self.quantized and
+                self.n_classes >= self.MANY_CLASSES and
                 self.n_rows * self.n_classes >= self.MANY_LOGITS and
                 self.dtype == torch.float32 and
                 self.X.dtype == torch.float32 and
@@ -527,6 +536,8 @@ class LinearClassLogits(object):
         return torch.stack(rows).reshape(lead + (self.n_rows,))
 
     def dense(self):
+        if self.quantized:
+            return _ops.quantized_linear(self.w, self.X, dtype=torch.float32)
         return torch.matmul(self.X, self.w.transpose(-1, -2))
 
 

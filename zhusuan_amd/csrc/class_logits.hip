@@ -39,12 +39,6 @@ __device__ __forceinline__ float bf16_value(uint16_t b) {
   return __builtin_bit_cast(float, (uint32_t)b << 16);
 }
 
-// what float16 leaves of x (nothing of an infinity)
-__device__ __forceinline__ float f16_rest(float x) {
-  const float h = (float)(_Float16)x;
-  return fabsf(h) == __builtin_inff() ? 0.f : x - h;
-}
-
 // ---- operands as the tile loop wants them ------------------------------------
 // The power of two that brings a magnitude near 2^14: 2^(its exponent - 13), 2^-113
 // and more, so that the reciprocal is a number; 1 for zeros and what is no number.
@@ -253,7 +247,7 @@ struct ClassArgs {
 // how r is written
 template <int F32>
 using ResidAs = typename std::conditional<
-    F32 == 0, AsBf16, typename std::conditional<F32 == 1, AsF32, AsF16>::type>::type;
+    F32 == 0, AsBf16, typename std::conditional<F32 == 1, AsF32, AsF16Planes>::type>::type;
 
 // LDS behind the tile loop: what the epilogue exchanges; behind that the tile's
 // biases and their gradient's column sums
@@ -341,7 +335,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
       else if (n < p.n) {
         if (EPI != kEpiStore) unit_n[j] = near_2_14(p.row_x[n]);
         if (EPI == kEpiStore) unit_n[j] = near_2_14(p.g[n]);
-        if (EPI == kEpiResidual) unit_r[j] = near_2_14(p.g[n]);
+        if (EPI == kEpiResidual) unit_r[j] = 1.f / near_2_14(p.g[n]);
       }
     }
   }
@@ -354,14 +348,14 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
       }
     };
     if (F32 == 0 && p.out_bf16) {
-      tile_rows<C, AsBf16>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+      tile_rows<C, AsBf16>(smem, lane, wave, value, [&](int, int n, int m, const tu4& piece) {
         if (n0 + n < p.n && m0 + m < p.m)
           store_piece(static_cast<uint16_t*>(p.out) + (n0 + n) * p.out_ld + m0 + m,
                       p.m - m0 - m, piece);
       });
     } else {
       float* out = static_cast<float*>(p.out) + (int64_t)blockIdx.y * p.out_split;
-      tile_rows<C, AsF32>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+      tile_rows<C, AsF32>(smem, lane, wave, value, [&](int, int n, int m, const tu4& piece) {
         if (n0 + n >= p.n || m0 + m >= p.m) return;
         float* o = out + (n0 + n) * p.out_ld + m0 + m;
         tu4 sum = piece;
@@ -457,64 +451,55 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
         p.part[(int64_t)tm * p.n + n0 + i] = t;
       }
     } else {
-      // r; of two planes one at a time, the second computing r again rather than
-      // keeping it
       float sum[C::WM][16];                // over the wave's rows, for the bias
       float* scol = sbias + C::BM;         // [WGN][BM]
-#pragma unroll 1
-      for (int pl = 0; pl < (F32 == 2 ? 2 : 1); ++pl) {
-        if (pl) __syncthreads();           // the plane before has been read
-        auto write = [&](auto BIASED) {
-          auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
-            constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
-            logits(I, J, Q, BIASED, v);
+      auto write = [&](auto BIASED) {
+        auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
+          constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
+          logits(I, J, Q, BIASED, v);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = ginv[j] * fast_exp(v[r] - mx[j]);
-            if (near[j]) {
+          for (int r = 0; r < 4; ++r) v[r] = ginv[j] * fast_exp(v[r] - mx[j]);
+          if (near[j]) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (yl[j] == i * 32 + acc_row(4 * q + r, half)) v[r] += g[j];
-            }
-            if (decltype(BIASED)::value && pl == 0 && p.bias_part) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
-            }
-            if (F32 == 2) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                v[r] *= 1.f / unit_r[j];
-                v[r] = pl == 0 ? v[r] : f16_rest(v[r]);
-              }
-            }
-          };
-          typedef ResidAs<F32> As;
-          tile_rows<C, As>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
-            const int64_t byte = (m0 + m) * (int)sizeof(typename As::T);
-            if (n0 + n < p.n && byte < p.resid_pitch)
-              *reinterpret_cast<tu4*>(p.resid + pl * p.resid_plane + (n0 + n) * p.resid_pitch +
-                                      byte) = piece;
-          });
-        };
-        if (biased)
-          write(std::true_type{});
-        else
-          write(std::false_type{});
-        if (pl == 0 && p.bias_part) {
-          blocks([&](auto I, auto Q) {
-            constexpr int i = decltype(I)::value, q = decltype(Q)::value;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float s = group_sum<32>(sum[i][4 * q + r]);
-              if (col == 0) scol[wn * C::BM + mw + i * 32 + acc_row(4 * q + r, half)] = s;
-            }
-          });
-          __syncthreads();
-          for (int i = threadIdx.x; i < C::BM; i += 256) {
-            float s = 0.f;
-#pragma unroll
-            for (int k = 0; k < C::WGN; ++k) s += scol[k * C::BM + i];
-            if (m0 + i < p.m) p.bias_part[(int64_t)tn * p.bias_ld + p.class0 + m0 + i] = s;
+            for (int r = 0; r < 4; ++r)
+              if (yl[j] == i * 32 + acc_row(4 * q + r, half)) v[r] += g[j];
           }
+          if (decltype(BIASED)::value && p.bias_part) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
+          }
+          if (F32 == 2) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] *= unit_r[j];
+          }
+        };
+        typedef ResidAs<F32> As;
+        tile_rows<C, As>(smem, lane, wave, value, [&](int plane, int n, int m, const tu4& piece) {
+          const int64_t byte = (m0 + m) * (int)sizeof(typename As::T);
+          if (n0 + n < p.n && byte < p.resid_pitch)
+            *reinterpret_cast<tu4*>(p.resid + plane * p.resid_plane + (n0 + n) * p.resid_pitch +
+                                    byte) = piece;
+        });
+      };
+      if (biased)
+        write(std::true_type{});
+      else
+        write(std::false_type{});
+      if (p.bias_part) {
+        blocks([&](auto I, auto Q) {
+          constexpr int i = decltype(I)::value, q = decltype(Q)::value;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float s = group_sum<32>(sum[i][4 * q + r]);
+            if (col == 0) scol[wn * C::BM + mw + i * 32 + acc_row(4 * q + r, half)] = s;
+          }
+        });
+        __syncthreads();
+        for (int i = threadIdx.x; i < C::BM; i += 256) {
+          float s = 0.f;
+#pragma unroll
+          for (int k = 0; k < C::WGN; ++k) s += scol[k * C::BM + i];
+          if (m0 + i < p.m) p.bias_part[(int64_t)tn * p.bias_ld + p.class0 + m0 + i] = s;
         }
       }
     }

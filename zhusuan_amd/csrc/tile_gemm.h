@@ -81,6 +81,11 @@ __device__ __forceinline__ uint32_t f16_pair(float a, float b) {
   const pair p = {(_Float16)a, (_Float16)b};
   return __builtin_bit_cast(uint32_t, p);
 }
+// what float16 leaves of x (nothing of an infinity)
+__device__ __forceinline__ float f16_rest(float x) {
+  const float h = (float)(_Float16)x;
+  return fabsf(h) == __builtin_inff() ? 0.f : x - h;
+}
 
 // kBytes: of an element of a k-major operand
 struct MmaBf16 {
@@ -425,7 +430,7 @@ __device__ __forceinline__ void tile_of_block(uint32_t bid, uint32_t n_wg, uint3
 
 // 256 x 256 tiles (one workgroup a CU) or 128 x 128 (two)?  And, for a product whose
 // k may be split with the parts joined afterwards, over how many workgroups?  What
-// takes the fewest of a large tile's steps (0.9 us): a CU's two small tiles take 0.58
+// takes the fewest of a large tile's steps (1.6 us): a CU's two small tiles take 0.58
 // of a large one's time (1140 against 1330 TFLOP/s); a tile's start and end cost eight
 // steps, and no share is shorter than that; parts are written and read by a launch of
 // their own.
@@ -448,7 +453,7 @@ inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, bool may_split, 
     for (int64_t s = 1; s <= most; s = s < most && 2 * s > most ? most : 2 * s) {
       const double rounds = (double)((tiles * s + slots - 1) / slots);
       const double t = rounds * (big ? 1.0 : 0.58) * (double)((steps + s - 1) / s + 8) +
-                       (s > 1 ? 5.0 + 2e-6 * (double)(m * n * s) : 0.0);
+                       (s > 1 ? 3.0 + 1.1e-6 * (double)(m * n * s) : 0.0);
       if ((big == 0 && s == 1) || t < least) {
         least = t;
         best = TilePlan{big != 0, (int)s};
@@ -484,29 +489,35 @@ __device__ __forceinline__ int acc_get(const ti16& v, int r) {
 // WGN x 32 rows of BM values are written as elements T (float, or bfloat16 bits),
 // 16 bytes between rows so that they start in different banks, and read back
 // in 16-byte pieces; two regions alternate, one barrier a block column.
-// As: how a value is written (AsF32, AsBf16, AsF16).
+// As: how a value is written (AsF32, AsBf16, or AsF16Planes: two rows, what float16
+// holds of it and the rest).
 //   value(i, j, q, v): the four values of registers 4 q .. 4 q + 3 of block (i, j)
-//   emit(n, m, piece): 16 bytes of row n (of the tile) from column m on
+//   emit(plane, n, m, piece): 16 bytes of row n (of the tile) from column m on
 struct AsF32 {
   typedef float T;
-  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
+  static constexpr int kPlanes = 1;
+  static __device__ __forceinline__ void put(char* to, int, const float (&v)[4]) {
     *reinterpret_cast<tf4*>(to) = tf4{v[0], v[1], v[2], v[3]};
   }
 };
 struct AsBf16 {
   typedef uint16_t T;
-  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
+  static constexpr int kPlanes = 1;
+  static __device__ __forceinline__ void put(char* to, int, const float (&v)[4]) {
     *reinterpret_cast<tu2*>(to) = tu2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
   }
 };
-struct AsF16 {
+struct AsF16Planes {
   typedef uint16_t T;
-  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
+  static constexpr int kPlanes = 2;
+  static __device__ __forceinline__ void put(char* to, int plane, const float (&v)[4]) {
     *reinterpret_cast<tu2*>(to) = tu2{f16_pair(v[0], v[1]), f16_pair(v[2], v[3])};
+    *reinterpret_cast<tu2*>(to + plane) = tu2{f16_pair(f16_rest(v[0]), f16_rest(v[1])),
+                                              f16_pair(f16_rest(v[2]), f16_rest(v[3]))};
   }
 };
 template <typename C, typename As>
-constexpr int kTileRowsLds = 2 * C::WGN * 32 * (C::BM * (int)sizeof(typename As::T) + 16);
+constexpr int kTileRowsLds = 2 * As::kPlanes * C::WGN * 32 * (C::BM * (int)sizeof(typename As::T) + 16);
 
 template <typename C, typename As, typename V, typename E>
 __device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& value, E&& emit) {
@@ -518,22 +529,26 @@ __device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& va
                      ((wave / C::WGN) * C::WM * 32 + 4 * half) * (int)sizeof(T);
   tile_for<C::WN>([&](auto J) {
     constexpr int j = decltype(J)::value;
-    constexpr int region = (j & 1) * kRows * kPitch;
+    constexpr int region = (j & 1) * As::kPlanes * kRows * kPitch;
     tile_for<C::WM>([&](auto I) {
       constexpr int i = decltype(I)::value;
       tile_for<4>([&](auto Q) {
         constexpr int q = decltype(Q)::value;
         float v[4];
         value(I, J, Q, v);
-        As::put(mine + region + (i * 32 + 8 * q) * (int)sizeof(T), v);
+        As::put(mine + region + (i * 32 + 8 * q) * (int)sizeof(T), kRows * kPitch, v);
       });
     });
     __syncthreads();
-    for (int c = threadIdx.x; c < kRows * kPieces; c += 256) {
-      const int row = c / kPieces, piece = c % kPieces;
-      emit((row >> 5) * C::WN * 32 + j * 32 + (row & 31), piece * kPer,
-           *reinterpret_cast<const tu4*>(smem + region + row * kPitch + piece * 16));
-    }
+    tile_for<As::kPlanes>([&](auto P) {
+      constexpr int plane = decltype(P)::value;
+      for (int c = threadIdx.x; c < kRows * kPieces; c += 256) {
+        const int row = c / kPieces, piece = c % kPieces;
+        emit(plane, (row >> 5) * C::WN * 32 + j * 32 + (row & 31), piece * kPer,
+             *reinterpret_cast<const tu4*>(smem + region + plane * kRows * kPitch +
+                                           row * kPitch + piece * 16));
+      }
+    });
   });
 }
 

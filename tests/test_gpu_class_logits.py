@@ -310,6 +310,62 @@ def test_captured_and_replayed(dtype):
         torch.randn(1000, 1000, device='cuda').sum().item()
 
 
+def test_two_graphs_replayed_in_turn():
+    """Two captured calls of different sizes, replayed interleaved and on two
+    streams: neither's workspace is the other's."""
+    sets = [problem(150, 64, 2000, torch.float32, 60, True, IGNORE),
+            problem(300, 96, 1200, torch.bfloat16, 61, True, IGNORE)]
+    graphs, outs, refs = [], [], []
+    for w, X, y, b, g in sets:
+        w, X, b = (t.requires_grad_() for t in (w, X, b))
+
+        def step():
+            lp = zs.linear_categorical_log_prob(w, X, y, bias=b,
+                                                ignore_label=IGNORE)
+            return (lp.detach(),) + torch.autograd.grad(lp, (w, X, b), g)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            refs.append([t.clone() for t in step()])
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append(graph)
+        outs.append(out)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, refs):
+            for a, c in zip(out, ref):
+                assert torch.equal(a, c)
+
+
+def test_units_of_operands_at_both_ends_of_the_range():
+    """float32 operands whose product is an ordinary number while each is near
+    the end of its range, either way round, and second derivatives refused."""
+    w, X, y, b, g = problem(300, 96, 700, torch.float32, 62)
+    for k in (2.0 ** 110, 2.0 ** -90):
+        lp, grads = run(w * k, X / k, y, None, g)
+        ref, refs = run(w, X, y, None, g)
+        # powers of two: nothing rounds differently, but for results below
+        # 2^-126, which float32 holds in multiples of 2^-149: 2^-150 off, in
+        # each of at most 64 parts that are joined
+        assert torch.equal(lp, ref)
+        for got, c, r in ((grads[0], k, refs[0]), (grads[1], 1 / k, refs[1])):
+            off = (got.double() * c - r.double()).abs()
+            assert bool((off <= 64 * 2.0 ** -150 * c).all())
+    X = X.requires_grad_()
+    lp = zs.linear_categorical_log_prob(w, X, y)
+    gx, = torch.autograd.grad(lp.sum(), X, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gx.square().sum(), X)
+
+
 def test_categorical_over_many_classes_takes_them_in_pieces():
     """Categorical(linear_class_logits(w, X)) of two chains: log_prob and its
     gradients, without the [2, N, V] logits."""

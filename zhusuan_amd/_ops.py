@@ -1083,6 +1083,7 @@ class ClassLogProb(_Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
         w, X, y, b, stats = ctx.saved_tensors
         (w2, _), (x2, _) = _rows_2d(w), _rows_2d(X)
@@ -1157,6 +1158,9 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
                          "one device")
     if ignore_label is not None:
         ignore_label = int(ignore_label)
+        if not -2 ** 63 <= ignore_label < 2 ** 63:
+            raise ValueError("linear_categorical_log_prob: ignore_label {} is "
+                             "no int64".format(ignore_label))
     flat = X.dim() == 2
     x2 = X if flat else X.reshape(-1, X.shape[-1])
     y = labels if flat else labels.reshape(-1)

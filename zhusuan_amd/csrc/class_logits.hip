@@ -40,13 +40,12 @@ __device__ __forceinline__ float bf16_value(uint16_t b) {
 }
 
 // ---- operands as the tile loop wants them ------------------------------------
-// The power of two that brings a magnitude near 2^14: 2^(its exponent - 13), 2^-113
-// and more, so that the reciprocal is a number; 1 for zeros and what is no number.
-__device__ __forceinline__ float near_2_14(float x) {
-  int e = (int)(__builtin_bit_cast(uint32_t, fabsf(x)) >> 23) - 127;
-  if (x == 0.f || e == 128) return 1.f;
-  e = e < -100 ? -100 : e;
-  return __builtin_bit_cast(float, (uint32_t)(e - 13 + 127) << 23);
+// The power of two that a magnitude near 2^14 is away from x, as its exponent (with
+// ldexp every one of them can be applied); 0 for zeros and what is no number.
+__device__ __forceinline__ int above_2_14(float x) {
+  const int e = (int)(__builtin_bit_cast(uint32_t, fabsf(x)) >> 23);
+  if (x == 0.f || e == 255) return 0;
+  return (e == 0 ? 1 : e) - 127 - 13;
 }
 
 // Rows to be packed, and the largest finite magnitudes that their scales come from:
@@ -68,7 +67,7 @@ struct PackArgs {
   PackJob job[3];
   int64_t pitch, ignore;
   const float* part;               // [3][kMaxParts]
-  float* scale;                    // [3]
+  int* scale;                      // [3]: exponents, see above_2_14
   float* row_max;                  // [rows of X]
 };
 
@@ -128,7 +127,7 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
 
 // blockIdx.y's rows of `cols` elements -> rows of `pitch` bytes, zero behind the
 // last column: elements as they are, or (SPLIT) float32 as two float16 planes of x /
-// scale, the row's or all rows'.  Rows whose label is `ignore` become zeros (whatever they hold, NaN
+// 2^e, the row's e or all rows'.  Rows whose label is `ignore` become zeros (whatever they hold, NaN
 // included, reaches no product).
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
   const PackJob& j = a.job[blockIdx.y];
   const int64_t groups = a.pitch / 16, total = j.rows * groups, plane = j.rows * a.pitch;
   if ((int64_t)blockIdx.x * 256 >= total) return;
-  float inv = 1.f, inv_g = 1.f;
+  int all = 0, all_g = 0;
   if (SPLIT) {
     __shared__ float s[2][4];
     float mx = 0.f, mg = 0.f;
@@ -154,13 +153,11 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
       s[1][threadIdx.x >> 6] = mg;
     }
     __syncthreads();
-    const float scale = near_2_14(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])));
-    const float scale_g = near_2_14(fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    inv = 1.f / scale;
-    inv_g = 1.f / scale_g;
+    all = above_2_14(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])));
+    all_g = above_2_14(fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     if (j.writes && blockIdx.x == 0 && threadIdx.x == 0) {
-      a.scale[j.part] = scale;
-      if (j.part_g != j.part) a.scale[j.part_g] = scale_g;
+      a.scale[j.part] = all;
+      if (j.part_g != j.part) a.scale[j.part_g] = all_g;
     }
   }
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
@@ -181,14 +178,12 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
     }
     unsigned char* const to = j.dst + r * a.pitch + (i - r * groups) * 16;
     if constexpr (SPLIT) {
-      // (powers of two: the products are exact)
-      const float f = j.row_max ? 1.f / near_2_14(j.row_max[r])
-                      : j.row_g ? inv_g * near_2_14(j.row_g[r]) : 1.f;
-      const float one = j.row_max ? 1.f : inv;
+      const int e = j.row_max ? above_2_14(j.row_max[r])
+                    : j.row_g ? all + all_g - above_2_14(j.row_g[r]) : all;
       tu4 hi, lo;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float x = v[2 * q] * one * f, y = v[2 * q + 1] * one * f;
+        const float x = ldexpf(v[2 * q], -e), y = ldexpf(v[2 * q + 1], -e);
         hi[q] = f16_pair(x, y);
         lo[q] = f16_pair(f16_rest(x), f16_rest(y));
       }
@@ -237,10 +232,11 @@ struct ClassArgs {
   void* out;
   int64_t out_ld, out_split;       // elements; split s at out + s * out_split
   int out_bf16, accumulate;
-  // float32 as planes: what the accumulators count in is *scale_m * *scale_n of
-  // the operands' units; in place of *scale_n a row of X has near_2_14(row_x[n]), and
-  // a row of r, in a product over the classes (row_units), near_2_14(g[n])
-  const float *scale_m, *scale_n, *row_x;
+  // float32 as planes: what the accumulators count in is 2^(*scale_m + *scale_n); in
+  // place of *scale_n a row of X has above_2_14(row_x[n]), and a row of r, in a product
+  // over the classes (row_units), above_2_14(g[n])
+  const int *scale_m, *scale_n;
+  const float* row_x;
   int row_units;
 };
 
@@ -321,22 +317,22 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
   }
 
   // what an accumulator counts in: planes of scaled operands
-  float unit_m = 1.f;
-  float unit_n[C::WN], unit_r[C::WN];
+  int unit[C::WN], unit_r[C::WN];
+  float unit_l[C::WN];
   if (F32 == 2) {
-    unit_m = *p.scale_m;
     const bool rows = EPI == kEpiStore && !p.row_units;
 #pragma unroll
     for (int j = 0; j < C::WN; ++j) {
       const int64_t n = n0 + nw + j * 32 + col;
-      unit_n[j] = unit_r[j] = 1.f;
+      unit[j] = *p.scale_m;
+      unit_r[j] = 0;
       if (rows)
-        unit_n[j] = *p.scale_n;
+        unit[j] += *p.scale_n;
       else if (n < p.n) {
-        if (EPI != kEpiStore) unit_n[j] = near_2_14(p.row_x[n]);
-        if (EPI == kEpiStore) unit_n[j] = near_2_14(p.g[n]);
-        if (EPI == kEpiResidual) unit_r[j] = 1.f / near_2_14(p.g[n]);
+        unit[j] += above_2_14(EPI == kEpiStore ? p.g[n] : p.row_x[n]);
+        if (EPI == kEpiResidual) unit_r[j] = -above_2_14(p.g[n]);
       }
+      unit_l[j] = ldexpf(1.f, unit[j]);
     }
   }
   if constexpr (EPI == kEpiStore) {
@@ -344,7 +340,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         v[r] = acc_get(acc[decltype(I)::value][decltype(J)::value], 4 * decltype(Q)::value + r);
-        if (F32 == 2) v[r] = v[r] * unit_m * unit_n[decltype(J)::value];
+        if (F32 == 2) v[r] = ldexpf(v[r], unit[decltype(J)::value]);
       }
     };
     if (F32 == 0 && p.out_bf16) {
@@ -391,7 +387,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         l[r] = acc_get(acc[i][j], 4 * q + r);
-        if (F32 == 2) l[r] = l[r] * unit_m * unit_n[j];
+        if (F32 == 2) l[r] *= unit_l[j];
         if (decltype(BIASED)::value) l[r] += bias[i][q][r];
       }
     };
@@ -470,7 +466,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
           }
           if (F32 == 2) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] *= unit_r[j];
+            for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], unit_r[j]);
           }
         };
         typedef ResidAs<F32> As;
@@ -646,6 +642,8 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   if (grad) {
     int64_t c = kPieceBytes / (resid_bytes * (q.n > 0 ? q.n : 1)) / 256 * 256;
     if (c < 4096) c = 4096;
+    // (a step's rows of r stay within the DMA's 32-bit offsets)
+    if (c > kMaxPitch / resid_bytes) c = kMaxPitch / resid_bytes;
     if (c < l.piece) l.piece = c;
   }
   l.pieces = tiles(q.v, l.piece);
@@ -778,7 +776,7 @@ int operands(const ClassProblem& q, const ClassLayout& l, unsigned char* ws,
   a.pitch = l.pitch;
   a.ignore = ignore;
   a.part = reinterpret_cast<const float*>(ws + l.maxima);
-  a.scale = reinterpret_cast<float*>(ws + l.scales);
+  a.scale = reinterpret_cast<int*>(ws + l.scales);
   a.row_max = reinterpret_cast<float*>(ws + l.row_max);
   int jobs = 0;
   int64_t most = 0;
@@ -883,7 +881,7 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   a.n = q.n;
   a.steps = (int)tiles(q.d * (l.whole ? 4 : 2), 128);
   a.terms = l.planes > 1 ? kTermsSplit : 1;
-  a.scale_m = reinterpret_cast<const float*>(ws + l.scales) + 1;
+  a.scale_m = reinterpret_cast<const int*>(ws + l.scales) + 1;
   a.row_x = reinterpret_cast<const float*>(ws + l.row_max);
   a.splits = 1;
   a.bias = bias;
@@ -931,7 +929,7 @@ extern "C" int zshmc_class_log_prob_grad(
   if (rc != ZSHMC_OK) return rc;
   const int terms = l.planes > 1 ? kTermsSplit : 1;
   const int64_t pb = l.whole ? 4 : 2;            // bytes of a plane's element
-  const float* scales = reinterpret_cast<const float*>(ws + l.scales);
+  const int* scales = reinterpret_cast<const int*>(ws + l.scales);
   const bool dx_joined = l.dx_splits * l.pieces > 1;
   for (int64_t c0 = 0; c0 < q.v; c0 += l.piece) {
     const int64_t c = q.v - c0 < l.piece ? q.v - c0 : l.piece;

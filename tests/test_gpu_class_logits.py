@@ -52,6 +52,21 @@ def test_several_pieces_of_the_vocabulary(dtype, N, V):
 
 
 @pytest.mark.parametrize('dtype', BOTH)
+@pytest.mark.parametrize('N,D,V', [
+    (1, 1024, 5), (7, 2816, 1029), (32, 1000, 500), (33, 1539, 640),
+    (128, 2048, 300), (300, 1200, 130)])
+def test_few_logits_of_many_features(N, D, V, dtype):
+    """Logits in parts, a share of the features each."""
+    for bias, ignore in ((False, None), (True, IGNORE)):
+        w, X, y, b, g = problem(N, D, V, dtype, N + D, bias, ignore)
+        if bias:
+            b[V // 2] = -float('inf')
+            y[y == V // 2] = 0
+            X[y == IGNORE] = float('nan')
+        check(w, X, y, b, g, ignore)
+
+
+@pytest.mark.parametrize('dtype', BOTH)
 def test_ignored_rows_may_hold_anything(dtype):
     w, X, y, b, g = problem(70, 96, 333, dtype, 5, True, IGNORE)
     clean = run(w, X, y, b, g, IGNORE)

@@ -19,8 +19,8 @@
 //
 // float32 operands go one of two ways.  Few rows: as they are, on
 // v_mfma_f32_32x32x2_f32.  More: as two float16 planes each (tile_gemm.h), of x /
-// 2^e with one e per operand (w, X, g), found by a pass over them; three products
-// on the 16-bit matrix cores are three times as fast.
+// 2^e with one e for w and g and one a row of X, found by a pass over them; three
+// products on the 16-bit matrix cores are three times as fast.
 #include "tile_gemm.h"
 
 namespace zshmc {
@@ -51,7 +51,7 @@ __device__ __forceinline__ int above_2_14(float x) {
 // Rows to be packed, and the largest finite magnitudes that their scales come from:
 // of each row of X (a row's logits are as good as its own values allow, whatever the
 // other rows hold), and of X, w and g per workgroup, without the rows (of X and g)
-// that are ignored.
+// that are ignored.  Bound by memory: 12 419 + 1021 rows of 784 float32 10 us, 4.0 TB/s.
 constexpr int kMaxParts = 1024;
 struct PackJob {
   const void* src;
@@ -127,8 +127,9 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
 
 // blockIdx.y's rows of `cols` elements -> rows of `pitch` bytes, zero behind the
 // last column: elements as they are, or (SPLIT) float32 as two float16 planes of x /
-// 2^e, the row's e or all rows'.  Rows whose label is `ignore` become zeros (whatever they hold, NaN
-// included, reaches no product).
+// 2^e, the row's e or all rows'.  Rows whose label is `ignore` become zeros (whatever
+// they hold, NaN included, reaches no product).  Bound by memory: the same rows into
+// planes 19 us, 4.5 TB/s of 4 bytes in and 4 out.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
   constexpr int N = SPLIT ? 8 : 16 / (int)sizeof(T);     // elements per 16 bytes out
@@ -253,6 +254,18 @@ constexpr int kEpiLds = EPI == kEpiStats      ? C::WGM * C::BN * 8
                                               : kTileRowsLds<C, AsF32>;
 
 // F32: 0 bfloat16, 1 float32 as it is, 2 float32 in planes
+//
+// Bound by the tile loop (tile_gemm.h) and, the fewer its steps, by what lies around
+// it: a workgroup's start, and an epilogue that takes e^x of every accumulator while
+// no MFMA runs (4 us of a 256 x 256 tile each).  bfloat16, 256 x 256 tiles:
+//   statistics  5000 x 1024 over 50 000 classes      542 us   945 TFLOP/s
+//               8192 x 4096 over 131 072            6610 us  1331
+//   r           4096 x 2048 over 32 768              570 us   965
+//   dw / dX     8192 x 4096, 16 384 classes a piece  832 / 908 us, 1322 / 1211
+// float32 in planes, 1021 x 784 over 12 419 classes (three products): statistics 71 us,
+// 842 TFLOP/s of float16; r 96 us, dw 88 us, dX 84 us.  One row of bfloat16 against
+// 32 768 x 4096 (tiles of 128 classes x 32 rows): 40 us, 6.7 TB/s; 100 rows of float32,
+// 12 419 x 128: 11 us, 28 TFLOP/s of the float32 matrix cores.
 template <typename C, int EPI, int F32>
 __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_kernel(
     ClassArgs p) {
@@ -503,7 +516,9 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 }
 
 // ---- joins ---------------------------------------------------------------------
-// ROWS rows x 256 / ROWS lanes of parts per workgroup
+// ROWS rows x 256 / ROWS lanes of parts per workgroup: few rows leave the chip empty
+// otherwise (1021 rows of 49 parts: 16 rows a workgroup 7 us, two 5); 5000 rows of 196
+// parts 7.5 us, 1.0 TB/s.
 template <int ROWS>
 __global__ __launch_bounds__(256) void join_stats_kernel(
     const cf2* __restrict__ part, int parts, const float* __restrict__ label_logit,
@@ -536,7 +551,46 @@ __global__ __launch_bounds__(256) void join_stats_kernel(
   if (stats) stats[row] = t;
 }
 
-// out[i] = sum of `parts` rows of x, in order
+// Logits in `splits` parts [n][classes] each, joined: per row and kStatClasses classes
+// (blockIdx.y, .x) their maximum and sum, and the label's logit.
+constexpr int kStatClasses = 1024;
+__global__ __launch_bounds__(256) void part_stats_kernel(
+    const float* __restrict__ parts, int splits, int64_t n_classes,
+    const float* __restrict__ bias, const int64_t* __restrict__ labels, cf2* __restrict__ part,
+    float* __restrict__ label_logit) {
+  const int64_t row = blockIdx.y, rows = gridDim.y, stride = rows * n_classes;
+  const int64_t y = labels[row];
+  float l[kStatClasses / 256];
+  float most = -__builtin_inff();
+#pragma unroll
+  for (int e = 0; e < kStatClasses / 256; ++e) {
+    const int64_t v = (int64_t)blockIdx.x * kStatClasses + e * 256 + threadIdx.x;
+    l[e] = -__builtin_inff();
+    if (v < n_classes) {
+      l[e] = sum_parts8(parts + row * n_classes + v, stride, splits);
+      if (bias) l[e] += bias[v];
+      if (v == y) label_logit[row] = l[e];
+    }
+    most = fmaxf(most, l[e]);
+  }
+  const float off = most == -__builtin_inff() ? 0.f : most;
+  cf2 t{most, 0.f};
+#pragma unroll
+  for (int e = 0; e < kStatClasses / 256; ++e) t[1] += fast_exp(l[e] - off);
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1) {
+    const float mx = __shfl_xor(t[0], step, 64), sum = __shfl_xor(t[1], step, 64);
+    t = join(t, cf2{mx, sum});
+  }
+  __shared__ cf2 red[4];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    part[blockIdx.x * rows + row] = join(join(red[0], red[1]), join(red[2], red[3]));
+}
+
+// out[i] = sum of `parts` rows of x, in order; bound by memory (4096 x 2048 of two
+// parts to bfloat16: 23 us, 3.6 TB/s)
 template <bool BF16>
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float* __restrict__ x, int parts,
                                                        int64_t stride, int64_t n,
@@ -564,7 +618,8 @@ unsigned grid_for(int64_t items) {
 }
 
 // bytes of r that one piece of classes may take: it is written, then read by
-// two products
+// two products, out of the 256 MB last-level cache as far as it fits.  8192 x 4096,
+// 131 072 classes, training: 64 MB 31.2 ms, 256 MB 27.6, 1 GB 27.5.
 constexpr int64_t kPieceBytes = 256ll << 20;
 constexpr int64_t kMaxPitch = 4ll << 20;
 
@@ -600,6 +655,8 @@ struct ClassLayout {
   int64_t xp, wp, xg;              // offsets; xg: X with its rows scaled like g's
   int64_t maxima, scales, row_max; // float32 in planes: of X, w, g; of X's rows
   int64_t part, label_logit;       // forward
+  int splits;                      // of the features; more than one: the parts
+  int64_t split_part;
   int tile;                        // see kTileClasses
   int64_t tiles_v;                 // parts of the statistics
   bool whole;                      // float32 operands as they are, no planes
@@ -659,6 +716,23 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
          tiles(l.piece, 128) * tiles(q.n, kTileRows[l.tile]) * 2 <= cus)
     ++l.tile;
   l.tiles_v = tiles(q.v, kTileClasses[l.tile]);
+  // Still half the chip or more without one, and many features: logits of a share of
+  // the features a workgroup, in parts, which a pass of its own joins.  float32 7 x
+  // 2816 over 4945 classes (39 tiles): 66 us whole, 24 in 8 parts
+  l.splits = 1;
+  l.split_part = 0;
+  const int64_t all_tiles = l.tiles_v * tiles(q.n, kTileRows[l.tile]);
+  const int64_t all_steps = tiles(q.d * element, 128);
+  if (!grad && l.tile == 3 && all_tiles > 0 && all_tiles * 2 <= cus) {
+    const int64_t room = 2 * cus / all_tiles;
+    l.splits = (int)(room < all_steps / 8 ? room : all_steps / 8);
+    if (l.splits < 2) l.splits = 1;
+    if (l.splits > 64) l.splits = 64;
+  }
+  if (l.splits > 1) {
+    l.split_part = take(l.splits * q.n * q.v * 4);
+    l.tiles_v = tiles(q.v, kStatClasses);
+  }
   l.part = l.label_logit = l.resid = l.dx_part = l.dw_part = l.bias_part = 0;
   if (!grad) {
     l.part = take(l.tiles_v * q.n * 8);
@@ -887,6 +961,23 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   a.bias = bias;
   a.labels = labels;
   a.n_classes = q.v;
+  if (l.splits > 1) {
+    a.splits = l.splits;
+    a.out = ws + l.split_part;
+    a.out_ld = q.v;
+    a.out_split = q.n * q.v;
+    a.g = a.row_x;                 // (the rows' units)
+    a.row_units = 1;
+    rc = l.planes > 1 ? launch_tile<Few<MmaF16, 1>, kEpiStore, 2>(a, s)
+         : l.whole    ? launch_tile<Few<MmaF32, 1>, kEpiStore, 1>(a, s)
+                      : launch_tile<Few<MmaBf16, 1>, kEpiStore, 0>(a, s);
+    if (rc != ZSHMC_OK) return rc;
+    hipLaunchKernelGGL(part_stats_kernel, dim3((unsigned)l.tiles_v, (unsigned)q.n), dim3(256), 0,
+                       s, static_cast<const float*>(a.out), l.splits, q.v, bias, labels, a.part,
+                       a.label_logit);
+    ZS_LAUNCH_CHECK("part_stats_kernel launch");
+    return join_stats(q, l, a, labels, has_ignore, ignore_label, log_prob, stats, s);
+  }
   rc = l.planes > 1 ? launch_logits<MmaF16, kEpiStats, 2>(a, l.tile, s)
        : l.whole    ? launch_logits<MmaF32, kEpiStats, 1>(a, l.tile, s)
                     : launch_logits<MmaBf16, kEpiStats, 0>(a, l.tile, s);

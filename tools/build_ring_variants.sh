@@ -11,7 +11,7 @@
 set -e
 cd "$(dirname "$0")/.."
 HIPCC=/opt/rocm/bin/hipcc
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p build/variants build/obj
 python -c "import __graft_entry__ as g; g.build()" >/dev/null
 while [ $# -ge 2 ]; do

@@ -1,6 +1,6 @@
 // Micro-benchmark: issue cost (cycles per wave64 instruction, one wave per
 // SIMD and 2 waves per SIMD) of the VALU instructions that dominate the
-// fused HMC kernel on gfx950.  Build: hipcc --offload-arch=gfx950 -O3 tools/instr_bench.hip -o build/instr_bench
+// fused HMC kernel on gfx950.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/instr_bench.hip -o build/instr_bench
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>
@@ -27,7 +27,6 @@
   f2 pa = {fa, fb}, pb = {fc, fd}, pc = {fb, fc}, pd = {fd, fa};
 
 KERNEL(k_fma, SETUP_ALL, asm volatile("v_fma_f32 %0, %0, %1, %2\n v_fma_f32 %1, %1, %2, %3\n v_fma_f32 %2, %2, %3, %0\n v_fma_f32 %3, %3, %0, %1" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd));)
-KERNEL(k_pk_fma, SETUP_ALL, asm volatile("v_pk_fma_f32 %0, %0, %1, %2\n v_pk_fma_f32 %1, %1, %2, %3\n v_pk_fma_f32 %2, %2, %3, %0\n v_pk_fma_f32 %3, %3, %0, %1" : "+v"(pa), "+v"(pb), "+v"(pc), "+v"(pd)); fa = pa[0];)
 KERNEL(k_xor, SETUP_ALL, asm volatile("v_xor_b32 %0, %0, %1\n v_xor_b32 %1, %1, %2\n v_xor_b32 %2, %2, %3\n v_xor_b32 %3, %3, %0" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_add_u32, SETUP_ALL, asm volatile("v_add_u32 %0, %0, %1\n v_add_u32 %1, %1, %2\n v_add_u32 %2, %2, %3\n v_add_u32 %3, %3, %0" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_alignbit, SETUP_ALL, asm volatile("v_alignbit_b32 %0, %0, %0, 13\n v_alignbit_b32 %1, %1, %1, 7\n v_alignbit_b32 %2, %2, %2, 5\n v_alignbit_b32 %3, %3, %3, 21" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
@@ -48,7 +47,6 @@ KERNEL(k_mul_i32_i24_pk, SETUP_ALL, asm volatile("v_mad_u32_u24 %0, %0, %1, %2\n
 KERNEL(k_xor_dep, SETUP_ALL, asm volatile("v_xor_b32 %0, %0, %1\n v_xor_b32 %0, %0, %2\n v_xor_b32 %0, %0, %3\n v_xor_b32 %0, %0, %1" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_xor_sgpr, SETUP_ALL, asm volatile("v_xor_b32 %0, s4, %0\n v_xor_b32 %1, s5, %1\n v_xor_b32 %2, s6, %2\n v_xor_b32 %3, s7, %3" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_xor_mad_mix, SETUP_ALL, asm volatile("v_mad_u64_u32 %0, vcc, %2, %3, 0\n v_xor_b32 %2, %2, %4\n v_xor_b32 %3, %3, %5\n v_mad_u64_u32 %1, vcc, %3, %2, 0\n v_xor_b32 %4, %4, %2\n v_xor_b32 %5, %5, %3" : "+v"(la), "+v"(lb), "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud) : : "vcc");)
-KERNEL(k_pk_xor_mix, SETUP_ALL, asm volatile("v_pk_fma_f32 %0, %0, %1, %2\n v_xor_b32 %4, %4, %5\n v_pk_fma_f32 %1, %1, %2, %3\n v_xor_b32 %5, %5, %6\n v_pk_fma_f32 %2, %2, %3, %0\n v_xor_b32 %6, %6, %7\n v_pk_fma_f32 %3, %3, %0, %1\n v_xor_b32 %7, %7, %4" : "+v"(pa), "+v"(pb), "+v"(pc), "+v"(pd), "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud)); fa = pa[0];)
 KERNEL(k_mov, SETUP_ALL, asm volatile("v_mov_b32 %0, %1\n v_mov_b32 %1, %2\n v_mov_b32 %2, %3\n v_mov_b32 %3, %0" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_mul_f32, SETUP_ALL, asm volatile("v_mul_f32 %0, %0, %1\n v_mul_f32 %1, %1, %2\n v_mul_f32 %2, %2, %3\n v_mul_f32 %3, %3, %0" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd));)
 KERNEL(k_add_dpp, SETUP_ALL, asm volatile("v_add_f32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:1\n v_add_f32_dpp %1, %1, %1 row_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:1\n v_add_f32_dpp %2, %2, %2 row_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:1\n v_add_f32_dpp %3, %3, %3 row_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:1" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd));)
@@ -58,7 +56,6 @@ KERNEL(k_cndmask_vccset, SETUP_ALL, asm volatile("s_mov_b64 vcc, 0x5555\n v_cndm
 KERNEL(k_cndmask_e64, SETUP_ALL, asm volatile("v_cndmask_b32_e64 %0, %0, %1, s[8:9]\n v_cndmask_b32_e64 %1, %1, %2, s[8:9]\n v_cndmask_b32_e64 %2, %2, %3, s[8:9]\n v_cndmask_b32_e64 %3, %3, %0, s[8:9]" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_cmp, SETUP_ALL, asm volatile("v_cmp_lt_f32 vcc, %0, %1\n v_cmp_lt_f32 vcc, %1, %2\n v_cmp_lt_f32 vcc, %2, %3\n v_cmp_lt_f32 vcc, %3, %0" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd) : : "vcc");)
 KERNEL(k_fma_sgpr, SETUP_ALL, asm volatile("v_fma_f32 %0, s4, %1, %0\n v_fma_f32 %1, s4, %2, %1\n v_fma_f32 %2, s4, %3, %2\n v_fma_f32 %3, s4, %0, %3" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd));)
-KERNEL(k_pk_fma_sgpr, SETUP_ALL, asm volatile("v_pk_fma_f32 %0, s[4:5], %1, %0\n v_pk_fma_f32 %1, s[4:5], %2, %1\n v_pk_fma_f32 %2, s[4:5], %3, %2\n v_pk_fma_f32 %3, s[4:5], %0, %3" : "+v"(pa), "+v"(pb), "+v"(pc), "+v"(pd)); fa = pa[0];)
 KERNEL(k_readlane, SETUP_ALL, asm volatile("v_readlane_b32 s8, %0, 63\n v_readlane_b32 s9, %1, 63\n v_readlane_b32 s10, %2, 63\n v_readlane_b32 s11, %3, 63" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud) : : "s8", "s9", "s10", "s11");)
 KERNEL(k_mov_dpp, SETUP_ALL, asm volatile("v_mov_b32_dpp %0, %1 row_bcast:15 row_mask:0xa bank_mask:0xf\n v_mov_b32_dpp %1, %2 row_bcast:15 row_mask:0xa bank_mask:0xf\n v_mov_b32_dpp %2, %3 row_bcast:15 row_mask:0xa bank_mask:0xf\n v_mov_b32_dpp %3, %0 row_bcast:15 row_mask:0xa bank_mask:0xf" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_mov_sgpr, SETUP_ALL, asm volatile("v_mov_b32 %0, s4\n v_mov_b32 %1, s5\n v_mov_b32 %2, s6\n v_mov_b32 %3, s7" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
@@ -68,7 +65,6 @@ KERNEL(k_mad_u64_sgpr, SETUP_ALL, asm volatile("v_mad_u64_u32 %0, vcc, s4, %3, 0
 KERNEL(k_sub_f32, SETUP_ALL, asm volatile("v_sub_f32 %0, %0, %1\n v_sub_f32 %1, %1, %2\n v_sub_f32 %2, %2, %3\n v_sub_f32 %3, %3, %0" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd));)
 KERNEL(k_lshr, SETUP_ALL, asm volatile("v_lshrrev_b32 %0, 8, %0\n v_lshrrev_b32 %1, 8, %1\n v_lshrrev_b32 %2, 8, %2\n v_lshrrev_b32 %3, 8, %3" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_sin2, SETUP_ALL, asm volatile("v_sin_f32 %0, %0\n v_cos_f32 %1, %1\n v_sqrt_f32 %2, %2\n v_log_f32 %3, %3" : "+v"(fa), "+v"(fb), "+v"(fc), "+v"(fd));)
-KERNEL(k_pk_mul, SETUP_ALL, asm volatile("v_pk_mul_f32 %0, %0, %1\n v_pk_mul_f32 %1, %1, %2\n v_pk_mul_f32 %2, %2, %3\n v_pk_mul_f32 %3, %3, %0" : "+v"(pa), "+v"(pb), "+v"(pc), "+v"(pd)); fa = pa[0];)
 
 KERNEL(k_bitop3, SETUP_ALL, asm volatile("v_bitop3_b32 %0, %0, %1, %2 bitop3:0x96\n v_bitop3_b32 %1, %1, %2, %3 bitop3:0x96\n v_bitop3_b32 %2, %2, %3, %0 bitop3:0x96\n v_bitop3_b32 %3, %3, %0, %1 bitop3:0x96" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
 KERNEL(k_bitop3_sgpr, SETUP_ALL, asm volatile("v_bitop3_b32 %0, %0, %1, s4 bitop3:0x96\n v_bitop3_b32 %1, %1, %2, s5 bitop3:0x96\n v_bitop3_b32 %2, %2, %3, s6 bitop3:0x96\n v_bitop3_b32 %3, %3, %0, s7 bitop3:0x96" : "+v"(ua), "+v"(ub), "+v"(uc), "+v"(ud));)
@@ -104,9 +100,9 @@ void run(const char* name, K kern, int waves_per_simd) {
 int main() {
   for (int w : {4}) {
 #define R(k) run(#k, k, w)
-    R(k_fma); R(k_pk_fma); R(k_xor); R(k_add_u32); R(k_mad_u64); R(k_log); R(k_cvt);
-    R(k_xor_dep); R(k_xor_sgpr); R(k_xor_mad_mix); R(k_pk_xor_mix); R(k_mov); R(k_mul_f32); R(k_add_dpp); R(k_cndmask);
-    R(k_cndmask_vccset); R(k_cndmask_e64); R(k_cmp); R(k_fma_sgpr); R(k_pk_fma_sgpr); R(k_readlane); R(k_mov_dpp); R(k_mov_sgpr); R(k_add_lit); R(k_xor_inl); R(k_mad_u64_sgpr); R(k_sub_f32); R(k_lshr); R(k_sin2); R(k_pk_mul);
+    R(k_fma); R(k_xor); R(k_add_u32); R(k_mad_u64); R(k_log); R(k_cvt);
+    R(k_xor_dep); R(k_xor_sgpr); R(k_xor_mad_mix); R(k_mov); R(k_mul_f32); R(k_add_dpp); R(k_cndmask);
+    R(k_cndmask_vccset); R(k_cndmask_e64); R(k_cmp); R(k_fma_sgpr); R(k_readlane); R(k_mov_dpp); R(k_mov_sgpr); R(k_add_lit); R(k_xor_inl); R(k_mad_u64_sgpr); R(k_sub_f32); R(k_lshr); R(k_sin2);
 #if 0
     R(k_mul_u24);
 #endif

@@ -21,6 +21,7 @@ import sys
 import tempfile
 
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-ffp-contract=fast',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-S', '--cuda-device-only']
 
 

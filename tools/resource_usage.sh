@@ -2,7 +2,7 @@
 # Per-kernel VGPR / spill / occupancy table of one HIP source.
 # Usage: tools/resource_usage.sh zhusuan_amd/csrc/hmc_fused_ring.hip [extra hipcc flags]
 src=$1; shift
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=fast -c "$src" -Rpass-analysis=kernel-resource-usage -o /dev/null "$@" 2>&1 |
+hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops -c "$src" -Rpass-analysis=kernel-resource-usage -o /dev/null "$@" 2>&1 |
   python3 -c '
 import re,sys
 name=None; row={}

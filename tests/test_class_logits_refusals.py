@@ -72,6 +72,7 @@ def test_class_log_prob_entry(lib):
         return lib.zshmc_class_log_prob_workspace(
             P, P, N, D, V, ldx, ldw, dtype, grad, 0, ctypes.addressof(n))
     assert ws() == 0 and n.value > 0
+    small = n.value
     assert ws(grad=1) == 0 and n.value > 0
     assert ws(N=0) == 0
     for bad in (dict(N=-1), dict(D=0), dict(V=0), dict(ldx=63), dict(ldw=1),

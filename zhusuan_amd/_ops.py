@@ -1078,6 +1078,7 @@ class ClassLogProb(_Function):
         y = labels.to(torch.int64).contiguous()
         out, stats, ctx.dims = _class_log_prob(w2, ldw, x2, ldx, y, b,
                                                ignore_label, True)
+        ctx.dtype = w.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.save_for_backward(w, X, y, b, stats)
         return out
@@ -1086,7 +1087,26 @@ class ClassLogProb(_Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
         w, X, y, b, stats = ctx.saved_tensors
-        (w2, _), (x2, _) = _rows_2d(w), _rows_2d(X)
+        # Saved-tensor hooks (save_on_cpu, a checkpoint's) may give back copies
+        # with other strides than the forward call saw, or other tensors
+        # altogether: what is read is described by what is here now.
+        N, D, V = ctx.dims[:3]
+        for t, shape, dtype in (
+                (w, (V, D), ctx.dtype), (X, (N, D), ctx.dtype),
+                (y, (N,), torch.int64), (b, (V,), _F32),
+                (stats, (N, 2), _F32)):
+            if t is not None and (tuple(t.shape) != shape or
+                                  t.dtype != dtype or
+                                  t.device != gout.device):
+                raise RuntimeError(
+                    "linear_categorical_log_prob: a saved tensor came back as "
+                    "{} {} on {}, {} {} on {} was saved".format(
+                        tuple(t.shape), t.dtype, t.device, shape, dtype,
+                        gout.device))
+        (w2, ldw), (x2, ldx) = _rows_2d(w), _rows_2d(X)
+        y, stats = y.contiguous(), stats.contiguous()
+        b = None if b is None else b.contiguous()
+        dims = (N, D, V, ldx, ldw) + ctx.dims[5:]
         need_w, need_x, _, need_b = ctx.needs_input_grad[:4]
         dev = X.device
         g = gout.to(_F32).contiguous()
@@ -1097,10 +1117,10 @@ class ClassLogProb(_Function):
         gb = torch.empty(w.shape[0], dtype=_F32, device=dev) \
             if need_b else None
         with _capi.on_device(dev) as stream:
-            n = _class_workspace_bytes(x2, w2, ctx.dims, 1)
+            n = _class_workspace_bytes(x2, w2, dims, 1)
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
             _capi.call('zshmc_class_log_prob_grad', x2.data_ptr(),
-                       w2.data_ptr(), _capi.ptr(b), y.data_ptr(), *ctx.dims,
+                       w2.data_ptr(), _capi.ptr(b), y.data_ptr(), *dims,
                        stats.data_ptr(), g.data_ptr(), _capi.ptr(gx),
                        _capi.ptr(gw), _capi.ptr(gb), ws.data_ptr(), n, stream)
         return (gw, gx, None, gb.to(ctx.bias_dtype) if need_b else None,

@@ -180,7 +180,8 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
     unsigned char* const to = j.dst + r * a.pitch + (i - r * groups) * 16;
     if constexpr (SPLIT) {
       const int e = j.row_max ? above_2_14(j.row_max[r])
-                    : j.row_g ? all + all_g - above_2_14(j.row_g[r]) : all;
+                    : j.row_g && j.row_g[r] != 0.f ? all + all_g - above_2_14(j.row_g[r])
+                                                   : all;   // (a row of r that is all zeros)
       tu4 hi, lo;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {

@@ -1029,7 +1029,8 @@ int zshmc_uni2_sample(int kind, float* out, const float* a, const float* b,
  *                  elements apart; bias [n_classes] float32 or NULL
  *   labels         int64; has_ignore: rows labelled `ignore_label` get 0 and
  *                  have no part in any gradient, whatever x holds there; any
- *                  other label outside [0, n_classes) gives NaN
+ *                  other label outside [0, n_classes) gives NaN, in the
+ *                  gradients only where grad_log_prob is not 0
  *   stats          [n_rows][2] float32 (maximum, sum of exponentials) for the
  *                  gradient, 8-byte aligned, or NULL
  *   workspace      16-byte aligned; its size from

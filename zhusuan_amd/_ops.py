@@ -1143,7 +1143,9 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
 
     A row labelled `ignore_label` has the log-probability 0 and no part in any
     gradient, whatever X holds there.  Any other label outside [0, V) gives
-    NaN (no host synchronisation to look for one).  Empty X is allowed."""
+    NaN (no host synchronisation to look for one), and gradients of NaN unless
+    its upstream gradient is 0 (a loss that masks the row).  Empty X is
+    allowed."""
     w, X, labels, bias = [
         _symbolic.force(t.tensor if hasattr(t, 'tensor') else t)
         for t in (w, X, labels, bias)]

@@ -309,7 +309,9 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
         if (EPI == kEpiResidual && !(p.has_ignore && label == p.ignore)) {
           const cf2 st = p.stats[n];
           mx[j] = st[0];
-          g[j] = label < 0 || label >= p.n_classes ? __builtin_nanf("") : p.g[n];
+          g[j] = p.g[n];
+          // (a label outside counts only where the caller lets the row count)
+          if ((label < 0 || label >= p.n_classes) && g[j] != 0.f) g[j] = __builtin_nanf("");
           ginv[j] = -g[j] / st[1];
         }
       }

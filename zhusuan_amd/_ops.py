@@ -1021,6 +1021,24 @@ def _rows_2d(t):
     return t2, ld if n > 1 else K
 
 
+def _no_tangents(what, *tensors):
+    """The kernels below have no forward-mode derivative: a dual tensor would
+    lose its tangent in them."""
+    unpack = torch.autograd.forward_ad.unpack_dual
+    if any(isinstance(t, torch.Tensor) and unpack(t).tangent is not None
+           for t in tensors):
+        raise NotImplementedError(what + ": has no forward-mode derivative")
+
+
+def _no_derivative(what, names, *tensors):
+    """... and those of 8-bit rows none at all."""
+    _no_tangents(what, *tensors)
+    if torch.is_grad_enabled() and any(
+            isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError("{}: has no gradient; detach {}, or call it under "
+                           "torch.no_grad()".format(what, names))
+
+
 _class_workspace = {}
 
 
@@ -1131,7 +1149,8 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
     """Log-probabilities of `labels` [...] under a Categorical whose logits
     are a linear map, `X @ w^T + bias`, for many classes: X [..., D] and
     w [V, D] float32 or bfloat16 (the same), integer labels of X's leading
-    shape, bias [V].  Returns float32 [...].  Differentiable in w, X and bias.
+    shape, bias [V].  Returns float32 [...].  Differentiable in w, X and bias
+    (in reverse mode, once).
 
     What `Categorical(logits=X @ w.T + bias).log_prob(labels)` computes, without the
     [..., V] logits: the classes are taken in pieces in both directions.
@@ -1176,6 +1195,7 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
         if tuple(bias.shape) != (w.shape[0],):
             raise ValueError("linear_categorical_log_prob: bias {} for {} "
                              "classes".format(tuple(bias.shape), w.shape[0]))
+    _no_tangents('linear_categorical_log_prob', w, X, bias)
     require_device(w, X, labels, bias)
     if w.device != X.device or labels.device != X.device or \
             (bias is not None and bias.device != X.device):
@@ -1280,8 +1300,9 @@ class QuantizedRows(object):
         return self._rows.device
 
     def dequantize(self, dtype=torch.float32):
-        """values * scale as a dense tensor."""
+        """values * scale as a dense tensor (no gradient)."""
         code = row_dtype(dtype, 'dequantize: dtype')
+        _no_derivative('dequantize', 'scale', self.scale)
         out = torch.empty(self._shape, dtype=dtype, device=self.device)
         n, K = self._rows.shape
         if n:
@@ -1296,7 +1317,9 @@ def quantize_rows(x):
     """x [..., K] (float32 or bfloat16) rounded to 8-bit integers with one
     scale per row, `scale = max|x| / 127` over the row and `values =
     rint(x / scale)` (to even): a `QuantizedRows`.  A row of zeros has the
-    scale 1; a row with an infinity or a NaN has the scale NaN.  No gradient."""
+    scale 1; a row with an infinity or a NaN has the scale NaN.  No gradient: an
+    x that requires one (a layer's weight) is refused while gradients are
+    recorded."""
     x = _symbolic.force(x.tensor if hasattr(x, 'tensor') else x)
     if not isinstance(x, torch.Tensor):
         raise TypeError("quantize_rows: a tensor expected")
@@ -1304,6 +1327,7 @@ def quantize_rows(x):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("quantize_rows: x [..., K] with K > 0 expected, got "
                          "{}".format(tuple(x.shape)))
+    _no_derivative('quantize_rows', 'x', x)
     require_device(x)
     x2, ldx = _rows_2d(x)
     n, K = x2.shape
@@ -1324,7 +1348,8 @@ def quantized_linear(w, X, bias=None, dtype=None):
     to 8 bits per row here -- or a `QuantizedRows`.  The integer sum is exact;
     out[..., v] = (scale_x scale_w[v]) * sum + bias[v] in float32, rounded once to
     `dtype` (X's own, float32 for a QuantizedRows).  K <= 131072.  No gradient:
-    an X or bias that requires one is refused while gradients are recorded."""
+    an X, bias or scale that requires one is refused while gradients are
+    recorded."""
     if not isinstance(w, QuantizedRows) or len(w._shape) != 2:
         raise TypeError("quantized_linear: w must be QuantizedRows [V, K]")
     X = _symbolic.force(X.tensor if hasattr(X, 'tensor') else X)
@@ -1350,15 +1375,11 @@ def quantized_linear(w, X, bias=None, dtype=None):
             raise ValueError("quantized_linear: bias must be a float tensor "
                              "[{}]".format(V))
         require_device(bias)
-        if bias.dtype != _F32 or not bias.is_contiguous():
-            bias = bias.to(_F32).contiguous()
     if X.device != w.device or (bias is not None and bias.device != w.device):
         raise ValueError("quantized_linear: all tensors must be on one device")
-    if torch.is_grad_enabled() and any(
-            isinstance(t, torch.Tensor) and t.requires_grad
-            for t in (X, bias)):
-        raise RuntimeError("quantized_linear: has no gradient; detach X and "
-                           "bias, or call it under torch.no_grad()")
+    _no_derivative('quantized_linear', 'X, bias and scales', bias, w.scale,
+                   X.scale if isinstance(X, QuantizedRows) else X)
+    bias = _float_row(bias)
     out = torch.empty(X.shape[:-1] + (V,), dtype=dtype, device=w.device)
     if not out.numel():
         return out

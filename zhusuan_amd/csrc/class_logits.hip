@@ -32,6 +32,9 @@ typedef float cf2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float fast_exp(float x) {
   return __builtin_amdgcn_exp2f(x * kLog2e);
 }
+__device__ __forceinline__ float only(uint32_t keep, float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & keep);
+}
 __device__ __forceinline__ uint16_t bf16_bits(float x) {
   return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
     for (int j = 0; j < C::WN; ++j) {
       const int64_t n = n0 + nw + j * 32 + col;
       yl[j] = -1;
-      // (a row behind the last one, or one that is ignored: r = 0 * e^-inf)
+      // (a row behind the last one, or one that is ignored: r = 0)
       mx[j] = 3e38f;
       g[j] = ginv[j] = 0.f;
       if (n < p.n) {
@@ -465,12 +468,17 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
     } else {
       float sum[C::WM][16];                // over the wave's rows, for the bias
       float* scol = sbias + C::BM;         // [WGN][BM]
+      // all bits, or none of a row that has no part: its logits need not be numbers (a
+      // row of zeros has NaN where a weight is infinite)
+      uint32_t keep[C::WN];
+#pragma unroll
+      for (int j = 0; j < C::WN; ++j) keep[j] = ginv[j] == 0.f ? 0u : ~0u;
       auto write = [&](auto BIASED) {
         auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
           constexpr int i = decltype(I)::value, j = decltype(J)::value, q = decltype(Q)::value;
           logits(I, J, Q, BIASED, v);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = ginv[j] * fast_exp(v[r] - mx[j]);
+          for (int r = 0; r < 4; ++r) v[r] = only(keep[j], ginv[j] * fast_exp(v[r] - mx[j]));
           if (near[j]) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)

@@ -1037,10 +1037,10 @@ int zshmc_uni2_sample(int kind, float* out, const float* a, const float* b,
  *                  zshmc_class_log_prob_workspace with the SAME pointers and
  *                  strides (gradient = 0 / 1 for the two calls), written to
  *                  *n_bytes_host.
- * float32 operands are multiplied as they are (few rows) or as two float16 planes
- * each: 22 bits and a sign of every element down to 2^-16 of the largest one of its
- * row of x (of w; for grad_w of x and grad_log_prob), and 2^-38 of the largest below
- * that.  Accumulation is float32. */
+ * float32 operands are multiplied as they are (few rows) or as three bfloat16
+ * planes each, which hold every bit of whatever is 2^-158 of the operand's
+ * largest element or more; the residual r that the gradients are products of
+ * is rounded to `dtype`.  Accumulation is float32. */
 int zshmc_class_log_prob_workspace(const void* x, const void* w,
                                    int64_t n_rows, int64_t n_features,
                                    int64_t n_classes, int64_t ldx, int64_t ldw,

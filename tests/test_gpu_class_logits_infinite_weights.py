@@ -21,7 +21,7 @@ def ours(w, X, y, b, g, ignore):
 @pytest.mark.parametrize('ignore', [None, IGNORE])
 @pytest.mark.parametrize('dtype,N', [
     (torch.bfloat16, 61), (torch.bfloat16, 301), (torch.bfloat16, 901),
-    (torch.float32, 61)])
+    (torch.float32, 61), (torch.float32, 301), (torch.float32, 901)])
 def test_infinite_weights_mask_a_class(dtype, N, ignore):
     """A constant feature whose weight is -inf (or the type's lowest) takes a
     class out, like a bias: the others' results are those without it."""
@@ -45,3 +45,18 @@ def test_infinite_weights_mask_a_class(dtype, N, ignore):
             assert torch.equal(got[0], ref[0])
             assert torch.equal(got[1], ref[1])
             assert torch.equal(got[3], ref[3])
+
+
+@pytest.mark.parametrize('N', [61, 301, 901])
+def test_an_infinite_feature_stays_in_its_row(N):
+    w, X, y, b, g = problem(N, 96, 700, torch.float32, 63, True)
+    ref = ours(w, X, y, b, g, None)
+    X2 = X.clone()
+    X2[2, 5], X2[40, 90] = float('inf'), -float('inf')
+    got = ours(w, X2, y, b, g, None)
+    bad = torch.zeros(N, dtype=torch.bool, device='cuda')
+    bad[2] = bad[40] = True
+    assert torch.equal(got[0].isnan(), bad)
+    assert torch.equal(got[0][~bad], ref[0][~bad])
+    assert torch.equal(got[2][~bad], ref[2][~bad])
+    assert bool(got[2][bad].isnan().all()) and bool(got[1].isnan().all())

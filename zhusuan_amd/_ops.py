@@ -1154,11 +1154,11 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
 
     What `Categorical(logits=X @ w.T + bias).log_prob(labels)` computes, without the
     [..., V] logits: the classes are taken in pieces in both directions.
-    bfloat16 operands are multiplied as they are, float32 ones as they are (few
-    rows) or in two parts, 22 bits and a sign of an element: as good as
-    float32's down to 2^-16 of the largest element of its row of X, or of w
-    (for w's gradient: of X), and to 2^-38 of that one below.  Sums and the
-    softmax statistics are float32 either way.
+    bfloat16 operands are multiplied as they are, and so is, rounded to
+    bfloat16, the residual r = g (one_hot - softmax) that dw and dX are products
+    of.  float32 operands, and r with them, keep all 24 bits: few rows as they
+    are, more in three bfloat16 parts (of elements down to 2^-158 of the
+    operand's largest).  Sums and the softmax statistics are float32 either way.
 
     A row labelled `ignore_label` has the log-probability 0 and no part in any
     gradient, whatever X holds there.  Any other label outside [0, V) gives

@@ -12,15 +12,14 @@
 // classes, each row's maximum and sum (8 bytes per row instead of 512 of
 // logits), and one pass that joins them.  Gradient: per piece of classes, the
 // logits again, turned into r in the epilogue (bfloat16, or for float32 operands
-// float32 or two float16 planes), then the two products over that piece; dX is
+// float32 or its planes), then the two products over that piece; dX is
 // accumulated in float32 over the pieces.  8 N V D flop for both directions,
 // six of them unavoidable.  M and S are float32; r is rounded to the operands'
 // precision because it is an operand of the matrix cores.
 //
 // float32 operands go one of two ways.  Few rows: as they are, on
-// v_mfma_f32_32x32x2_f32.  More: as two float16 planes each (tile_gemm.h), of x /
-// 2^e with one e for w and g and one a row of X, found by a pass over them; three
-// products on the 16-bit matrix cores are three times as fast.
+// v_mfma_f32_32x32x2_f32.  More: as three bfloat16 planes each (tile_gemm.h), which
+// hold every bit of them; six products on the 16-bit matrix cores are 1.3 times as fast.
 #include "tile_gemm.h"
 
 namespace zshmc {
@@ -38,40 +37,31 @@ __device__ __forceinline__ float only(uint32_t keep, float x) {
 __device__ __forceinline__ uint16_t bf16_bits(float x) {
   return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
-__device__ __forceinline__ float bf16_value(uint16_t b) {
-  return __builtin_bit_cast(float, (uint32_t)b << 16);
-}
 
 // ---- operands as the tile loop wants them ------------------------------------
-// The power of two that a magnitude near 2^14 is away from x, as its exponent (with
-// ldexp every one of them can be applied); 0 for zeros and what is no number.
-__device__ __forceinline__ int above_2_14(float x) {
-  const int e = (int)(__builtin_bit_cast(uint32_t, fabsf(x)) >> 23);
-  if (x == 0.f || e == 255) return 0;
-  return (e == 0 ? 1 : e) - 127 - 13;
+// An operand's unit 2^e: its largest magnitude x is near 2^48 units (see tile_gemm.h).
+// With ldexp every exponent can be applied; 0 for zeros.
+__device__ __forceinline__ int unit_of(float x) {
+  const int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23);
+  return x == 0.f ? 0 : (e == 0 ? 1 : e) - 127 - 48;
 }
 
-// Rows to be packed, and the largest finite magnitudes that their scales come from:
-// of each row of X (a row's logits are as good as its own values allow, whatever the
-// other rows hold), and of X, w and g per workgroup, without the rows (of X and g)
-// that are ignored.  Bound by memory: 12 419 + 1021 rows of 784 float32 10 us, 4.0 TB/s.
+// Rows to be packed, and the largest finite magnitudes that their units come from: of X,
+// w and g per workgroup, without the rows (of X and g) that are ignored.  Bound by
+// memory: 12 419 + 1021 rows of 784 float32 10 us, 4.0 TB/s.
 constexpr int kMaxParts = 1024;
 struct PackJob {
   const void* src;
   int64_t rows, cols, ld;
   unsigned char* dst;
   const int64_t* labels;           // rows labelled `ignore` become zeros; or NULL
-  const float* row_max;            // rows have a scale each: or NULL
-  const float* row_g;              // rows are scaled like g's: or NULL
-  int part, part_g;                // whose maximum
-  int writes;                      // the first workgroup writes scale[part] ( + [part_g])
 };
 struct PackArgs {
-  PackJob job[3];
+  PackJob job[2];                  // X, w (in planes both, else any that need it)
   int64_t pitch, ignore;
-  const float* part;               // [3][kMaxParts]
-  int* scale;                      // [3]: exponents, see above_2_14
-  float* row_max;                  // [rows of X]
+  const float* part;               // [3][kMaxParts]: of X, w, g
+  int* unit;                       // [3]
+  int has_g;
 };
 
 __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* __restrict__ g,
@@ -87,7 +77,10 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
     v = fabsf(v);
     mx = v <= 3.402823466e38f ? fmaxf(mx, v) : mx;
   };
-  auto four = [&](int64_t r, int64_t c) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = (i - r * groups) * 4;
+    if (j.labels && j.labels[r] == a.ignore) continue;
     const float* from = src + r * ld + c;
     if (c + 4 <= cols) {
       typedef float any __attribute__((ext_vector_type(4), aligned(4)));
@@ -96,27 +89,6 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
       for (int e = 0; e < 4; ++e) widen(v[e]);
     } else {
       for (int e = 0; e < cols - c; ++e) widen(from[e]);
-    }
-  };
-  if (k == 0) {                    // a wave a row
-    float all = 0.f;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows;
-         r += (int64_t)gridDim.x * 4) {
-      mx = 0.f;
-      if (!(j.labels && j.labels[r] == a.ignore))
-        for (int64_t c = (threadIdx.x & 63) * 4; c < cols; c += 256) four(r, c);
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-      if ((threadIdx.x & 63) == 0) a.row_max[r] = mx;
-      all = fmaxf(all, mx);
-    }
-    mx = all;
-  } else {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-         i += (int64_t)gridDim.x * 256) {
-      const int64_t r = i / groups;
-      if (j.labels && j.labels[r] == a.ignore) continue;
-      four(r, (i - r * groups) * 4);
     }
   }
 #pragma unroll
@@ -128,40 +100,41 @@ __global__ __launch_bounds__(256) void part_max_kernel(PackArgs a, const float* 
     part[k * kMaxParts + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 }
 
+// the parts' maximum, by a workgroup
+__device__ __forceinline__ float join_max(const float* __restrict__ part) {
+  __shared__ float s[4];
+  float mx = 0.f;
+  for (int i = threadIdx.x; i < kMaxParts; i += 256) mx = fmaxf(mx, part[i]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+
 // blockIdx.y's rows of `cols` elements -> rows of `pitch` bytes, zero behind the
-// last column: elements as they are, or (SPLIT) float32 as two float16 planes of x /
-// 2^e, the row's e or all rows'.  Rows whose label is `ignore` become zeros (whatever
-// they hold, NaN included, reaches no product).  Bound by memory: the same rows into
-// planes 19 us, 4.5 TB/s of 4 bytes in and 4 out.
+// last column: elements as they are, or (SPLIT) float32 as three bfloat16 planes of x /
+// 2^e.  Rows whose label is `ignore` become zeros (whatever they hold, NaN included,
+// reaches no product).  An infinite weight stands in the lowest plane alone, which meets
+// only the other operand's highest: in the highest it would meet the rest of x, of any
+// sign or 0.  (An infinite x makes its row NaN in either.)  Bound by memory: 12 419 + 1021
+// rows of 784 21 us, 5.0 TB/s of 4 bytes in and 6 out.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
   constexpr int N = SPLIT ? 8 : 16 / (int)sizeof(T);     // elements per 16 bytes out
   const PackJob& j = a.job[blockIdx.y];
   const int64_t groups = a.pitch / 16, total = j.rows * groups, plane = j.rows * a.pitch;
   if ((int64_t)blockIdx.x * 256 >= total) return;
-  int all = 0, all_g = 0;
+  int unit = 0;
   if (SPLIT) {
-    __shared__ float s[2][4];
-    float mx = 0.f, mg = 0.f;
-    for (int i = threadIdx.x; i < kMaxParts; i += 256) {
-      mx = fmaxf(mx, a.part[j.part * kMaxParts + i]);
-      mg = fmaxf(mg, a.part[j.part_g * kMaxParts + i]);
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-      mg = fmaxf(mg, __shfl_xor(mg, off, 64));
-    }
-    if ((threadIdx.x & 63) == 0) {
-      s[0][threadIdx.x >> 6] = mx;
-      s[1][threadIdx.x >> 6] = mg;
-    }
-    __syncthreads();
-    all = above_2_14(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])));
-    all_g = above_2_14(fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    if (j.writes && blockIdx.x == 0 && threadIdx.x == 0) {
-      a.scale[j.part] = all;
-      if (j.part_g != j.part) a.scale[j.part_g] = all_g;
+    unit = unit_of(join_max(a.part + blockIdx.y * kMaxParts));
+    if (blockIdx.x == 0) {
+      if (threadIdx.x == 0) a.unit[blockIdx.y] = unit;
+      if (a.has_g && blockIdx.y == 0) {
+        const int unit_g = unit_of(join_max(a.part + 2 * kMaxParts));
+        if (threadIdx.x == 0) a.unit[2] = unit_g;
+      }
     }
   }
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
@@ -182,18 +155,23 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
     }
     unsigned char* const to = j.dst + r * a.pitch + (i - r * groups) * 16;
     if constexpr (SPLIT) {
-      const int e = j.row_max ? above_2_14(j.row_max[r])
-                    : j.row_g && j.row_g[r] != 0.f ? all + all_g - above_2_14(j.row_g[r])
-                                                   : all;   // (a row of r that is all zeros)
-      tu4 hi, lo;
+      tu4 p[kPlanes];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float x = ldexpf(v[2 * q], -e), y = ldexpf(v[2 * q + 1], -e);
-        hi[q] = f16_pair(x, y);
-        lo[q] = f16_pair(f16_rest(x), f16_rest(y));
+        const float x = ldexpf(v[2 * q], -unit), y = ldexpf(v[2 * q + 1], -unit);
+        uint32_t w[kPlanes];
+        bf16_planes(x, y, w);
+        if (blockIdx.y == 1) {     // w
+          const uint32_t low = (fabsf(x) == __builtin_inff() ? 0xffffu : 0u) |
+                               (fabsf(y) == __builtin_inff() ? 0xffff0000u : 0u);
+          w[kPlanes - 1] |= w[0] & low;
+          w[0] &= ~low;
+        }
+#pragma unroll
+        for (int k = 0; k < kPlanes; ++k) p[k][q] = w[k];
       }
-      *reinterpret_cast<tu4*>(to) = hi;
-      *reinterpret_cast<tu4*>(to + plane) = lo;
+#pragma unroll
+      for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<tu4*>(to + k * plane) = p[k];
     } else {
       typedef T whole __attribute__((ext_vector_type(N)));
       whole w;
@@ -237,18 +215,13 @@ struct ClassArgs {
   void* out;
   int64_t out_ld, out_split;       // elements; split s at out + s * out_split
   int out_bf16, accumulate;
-  // float32 as planes: what the accumulators count in is 2^(*scale_m + *scale_n); in
-  // place of *scale_n a row of X has above_2_14(row_x[n]), and a row of r, in a product
-  // over the classes (row_units), above_2_14(g[n])
-  const int *scale_m, *scale_n;
-  const float* row_x;
-  int row_units;
+  // float32 in planes: the operands' units (their exponents); r is in units of g
+  const int *unit_a, *unit_b, *unit_g;
 };
 
-// how r is written
+// how r leaves through the LDS
 template <int F32>
-using ResidAs = typename std::conditional<
-    F32 == 0, AsBf16, typename std::conditional<F32 == 1, AsF32, AsF16Planes>::type>::type;
+using ResidAs = typename std::conditional<F32 == 0, AsBf16, AsF32>::type;
 
 // LDS behind the tile loop: what the epilogue exchanges; behind that the tile's
 // biases and their gradient's column sums
@@ -266,8 +239,8 @@ constexpr int kEpiLds = EPI == kEpiStats      ? C::WGM * C::BN * 8
 //               8192 x 4096 over 131 072            6610 us  1331
 //   r           4096 x 2048 over 32 768              570 us   965
 //   dw / dX     8192 x 4096, 16 384 classes a piece  832 / 908 us, 1322 / 1211
-// float32 in planes, 1021 x 784 over 12 419 classes (three products): statistics 71 us,
-// 842 TFLOP/s of float16; r 96 us, dw 88 us, dX 84 us.  One row of bfloat16 against
+// float32 in planes, 1021 x 784 over 12 419 classes (six products): statistics 131 us,
+// 913 TFLOP/s; r 154 us, dw 166 us, dX 161 us.  One row of bfloat16 against
 // 32 768 x 4096 (tiles of 128 classes x 32 rows): 40 us, 6.7 TB/s; 100 rows of float32,
 // 12 419 x 128: 11 us, 28 TFLOP/s of the float32 matrix cores.
 template <typename C, int EPI, int F32>
@@ -312,7 +285,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
         if (EPI == kEpiResidual && !(p.has_ignore && label == p.ignore)) {
           const cf2 st = p.stats[n];
           mx[j] = st[0];
-          g[j] = p.g[n];
+          g[j] = F32 == 2 ? ldexpf(p.g[n], -*p.unit_g) : p.g[n];
           // (a label outside counts only where the caller lets the row count)
           if ((label < 0 || label >= p.n_classes) && g[j] != 0.f) g[j] = __builtin_nanf("");
           ginv[j] = -g[j] / st[1];
@@ -335,42 +308,25 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
       for (int j = 0; j < C::WN; ++j) acc[i][j] = typename C::MMA::Acc{};
   }
 
-  // what an accumulator counts in: planes of scaled operands
-  int unit[C::WN], unit_r[C::WN];
-  float unit_l[C::WN];
-  if (F32 == 2) {
-    const bool rows = EPI == kEpiStore && !p.row_units;
-#pragma unroll
-    for (int j = 0; j < C::WN; ++j) {
-      const int64_t n = n0 + nw + j * 32 + col;
-      unit[j] = *p.scale_m;
-      unit_r[j] = 0;
-      if (rows)
-        unit[j] += *p.scale_n;
-      else if (n < p.n) {
-        unit[j] += above_2_14(EPI == kEpiStore ? p.g[n] : p.row_x[n]);
-        if (EPI == kEpiResidual) unit_r[j] = -above_2_14(p.g[n]);
-      }
-      unit_l[j] = ldexpf(1.f, unit[j]);
-    }
-  }
+  // what an accumulator counts in
+  const int unit = F32 == 2 ? *p.unit_a + *p.unit_b : 0;
   if constexpr (EPI == kEpiStore) {
     auto value = [&](auto I, auto J, auto Q, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         v[r] = acc_get(acc[decltype(I)::value][decltype(J)::value], 4 * decltype(Q)::value + r);
-        if (F32 == 2) v[r] = ldexpf(v[r], unit[decltype(J)::value]);
+        if (F32 == 2) v[r] = ldexpf(v[r], unit);
       }
     };
     if (F32 == 0 && p.out_bf16) {
-      tile_rows<C, AsBf16>(smem, lane, wave, value, [&](int, int n, int m, const tu4& piece) {
+      tile_rows<C, AsBf16>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
         if (n0 + n < p.n && m0 + m < p.m)
           store_piece(static_cast<uint16_t*>(p.out) + (n0 + n) * p.out_ld + m0 + m,
                       p.m - m0 - m, piece);
       });
     } else {
       float* out = static_cast<float*>(p.out) + (int64_t)blockIdx.y * p.out_split;
-      tile_rows<C, AsF32>(smem, lane, wave, value, [&](int, int n, int m, const tu4& piece) {
+      tile_rows<C, AsF32>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
         if (n0 + n >= p.n || m0 + m >= p.m) return;
         float* o = out + (n0 + n) * p.out_ld + m0 + m;
         tu4 sum = piece;
@@ -406,7 +362,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         l[r] = acc_get(acc[i][j], 4 * q + r);
-        if (F32 == 2) l[r] *= unit_l[j];
+        if (F32 == 2) l[r] = ldexpf(l[r], unit);
         if (decltype(BIASED)::value) l[r] += bias[i][q][r];
       }
     };
@@ -488,17 +444,23 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum[i][4 * q + r] = j ? sum[i][4 * q + r] + v[r] : v[r];
           }
-          if (F32 == 2) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], unit_r[j]);
-          }
         };
-        typedef ResidAs<F32> As;
-        tile_rows<C, As>(smem, lane, wave, value, [&](int plane, int n, int m, const tu4& piece) {
-          const int64_t byte = (m0 + m) * (int)sizeof(typename As::T);
-          if (n0 + n < p.n && byte < p.resid_pitch)
-            *reinterpret_cast<tu4*>(p.resid + plane * p.resid_plane + (n0 + n) * p.resid_pitch +
-                                    byte) = piece;
+        tile_rows<C, ResidAs<F32>>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
+          constexpr int kBytes = F32 == 1 ? 4 : 2;       // of a value in a plane
+          const int64_t byte = (m0 + m) * kBytes;
+          if (n0 + n >= p.n || byte >= p.resid_pitch) return;
+          unsigned char* const to = p.resid + (n0 + n) * p.resid_pitch + byte;
+          if constexpr (F32 == 2) {
+            const tf4 x = __builtin_bit_cast(tf4, piece);
+            uint32_t front[kPlanes], back[kPlanes];
+            bf16_planes(x[0], x[1], front);
+            bf16_planes(x[2], x[3], back);
+#pragma unroll
+            for (int k = 0; k < kPlanes; ++k)
+              *reinterpret_cast<tu2*>(to + k * p.resid_plane) = tu2{front[k], back[k]};
+          } else {
+            *reinterpret_cast<tu4*>(to) = piece;
+          }
         });
       };
       if (biased)
@@ -519,6 +481,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void class_tile_k
           float s = 0.f;
 #pragma unroll
           for (int k = 0; k < C::WGN; ++k) s += scol[k * C::BM + i];
+          if (F32 == 2) s = ldexpf(s, *p.unit_g);
           if (m0 + i < p.m) p.bias_part[(int64_t)tn * p.bias_ld + p.class0 + m0 + i] = s;
         }
       }
@@ -628,10 +591,10 @@ unsigned grid_for(int64_t items) {
   return (unsigned)(b < 1 ? 1 : b > 16384 ? 16384 : b);
 }
 
-// bytes of r that one piece of classes may take: it is written, then read by
-// two products, out of the 256 MB last-level cache as far as it fits.  8192 x 4096,
-// 131 072 classes, training: 64 MB 31.2 ms, 256 MB 27.6, 1 GB 27.5.
-constexpr int64_t kPieceBytes = 256ll << 20;
+// logits of one piece of classes: r is written, then read by two products (2 bytes a
+// logit, 6 in planes).  8192 x 4096, 131 072 classes, bfloat16, training: 2^25 31.2 ms,
+// 2^27 27.6, 2^29 27.5; float32 over 65 536 classes: 2^25.4 93.2, 2^26.4 89.2, 2^27 84.3.
+constexpr int64_t kPieceLogits = 1ll << 27;
 constexpr int64_t kMaxPitch = 4ll << 20;
 
 struct ClassProblem {
@@ -650,10 +613,12 @@ bool direct(const void* p, int64_t ld, const ClassProblem& q, bool whole) {
 }
 
 // Up to how many rows float32 operands are multiplied as they are, 2 N V D flop a
-// product at 140 TFLOP/s, rather than packed into planes: 12 bytes an element of w,
-// then three products at 1250.  They meet near 250 rows for the one product of the
-// forward call, near 80 for the three of the gradient's.
-constexpr int64_t kWholeRows = 256, kWholeRowsGrad = 80;
+// product at 140 TFLOP/s, rather than packed into planes: 14 bytes an element of w, then
+// six products at 1200.  As they are / in planes, us, D x V: forward, 784 x 12 419 of 512
+// rows 110 / 105, of 700 201 / 141; 4096 x 32 768 963 / 1006 and 1457 / 1688.  With the
+// gradients, 784 x 12 419 of 256 rows 243 / 283, of 400 423 / 379; 4096 x 32 768 2069 /
+// 2503 and 3803 / 3180.  (As they are, the matrix cores take what is below 2^-126 for 0.)
+constexpr int64_t kWholeRows = 512, kWholeRowsGrad = 256;
 
 // the logits' tiles: classes x rows of X
 constexpr int kTileClasses[] = {256, 128, 128, 128}, kTileRows[] = {256, 128, 64, 32};
@@ -663,8 +628,8 @@ struct ClassLayout {
   int64_t pitch;                   // of packed operands, bytes
   int64_t x_plane, w_plane, planes;
   bool pack_x, pack_w;
-  int64_t xp, wp, xg;              // offsets; xg: X with its rows scaled like g's
-  int64_t maxima, scales, row_max; // float32 in planes: of X, w, g; of X's rows
+  int64_t xp, wp;                  // offsets
+  int64_t maxima, units;           // float32 in planes: of X, w, g
   int64_t part, label_logit;       // forward
   int splits;                      // of the features; more than one: the parts
   int64_t split_part;
@@ -686,7 +651,7 @@ int clip(int splits, int64_t steps) { return (int)(splits < steps ? splits : ste
 ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
   ClassLayout l;
   l.whole = q.f32() && q.n <= (grad ? kWholeRowsGrad : kWholeRows);
-  l.planes = q.f32() && !l.whole ? 2 : 1;
+  l.planes = q.f32() && !l.whole ? kPlanes : 1;
   l.pitch = round_up(q.d * (l.whole ? 4 : 2), 128);
   l.pack_x = !direct(q.x, q.ldx, q, l.whole) || (grad && has_ignore);
   l.pack_w = !direct(q.w, q.ldw, q, l.whole);
@@ -700,22 +665,20 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     return here;
   };
   l.maxima = l.planes > 1 ? take(3ll * kMaxParts * 4) : 0;
-  l.scales = l.planes > 1 ? take(3 * 4) : 0;
-  l.row_max = l.planes > 1 ? take(q.n * 4) : 0;
+  l.units = l.planes > 1 ? take(3 * 4) : 0;
   l.xp = l.pack_x ? take(l.planes * l.x_plane) : 0;
   l.wp = l.pack_w ? take(l.planes * l.w_plane) : 0;
-  l.xg = grad && l.planes > 1 ? take(l.planes * l.x_plane) : 0;
-  const int64_t resid_bytes = q.f32() ? 4 : 2;
+  const int64_t element = l.whole ? 4 : 2;       // bytes of a plane's
   l.piece = q.v;
   if (grad) {
-    int64_t c = kPieceBytes / (resid_bytes * (q.n > 0 ? q.n : 1)) / 256 * 256;
+    int64_t c = kPieceLogits / (q.n > 0 ? q.n : 1) / 256 * 256;
     if (c < 4096) c = 4096;
     // (a step's rows of r stay within the DMA's 32-bit offsets)
-    if (c > kMaxPitch / resid_bytes) c = kMaxPitch / resid_bytes;
+    if (c > kMaxPitch / element) c = kMaxPitch / element;
     if (c < l.piece) l.piece = c;
   }
   l.pieces = tiles(q.v, l.piece);
-  const int64_t element = l.whole ? 4 : 2, terms = l.planes > 1 ? kTermsSplit : 1;
+  const int64_t terms = l.planes > 1 ? kTermsSplit : 1;
   l.tile = q.n <= 32                                            ? 3
            : q.n <= 64                                          ? 2
            : plan_tiles(l.piece, q.n, terms * tiles(q.d * element, 128), false, cus).big ? 0
@@ -749,17 +712,27 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
     l.part = take(l.tiles_v * q.n * 8);
     l.label_logit = take(q.n * 4);
   } else {
-    l.resid_pitch = round_up(l.piece * (l.whole ? 4 : 2), 128);
+    l.resid_pitch = round_up(l.piece * element, 128);
     l.resid_plane = q.n * l.resid_pitch;
     l.resid = take(l.planes * l.resid_plane);
-    const TilePlan dw = plan_tiles(l.piece, q.d, terms * tiles(q.n * element, 128), true, cus);
+    // (planes: shares of three k-steps, 18 steps, at least, or the parts grow past r)
+    const int64_t rows_k = tiles(q.n * element, 128), classes_k = tiles(l.piece * element, 128);
+    const int64_t least = l.planes > 1 ? 3 : 1;
+    const TilePlan dw = plan_tiles(l.piece, q.d, terms * rows_k, true, cus);
     l.dw_tile = dw.big ? 0 : 1;
-    l.dw_splits = clip(dw.splits, tiles(q.n * element, 128));
-    if (l.dw_splits > 1) l.dw_part = take(l.dw_splits * l.piece * q.d * 4);
-    const TilePlan dx = plan_tiles(q.n, q.d, terms * tiles(l.piece * element, 128), true, cus);
+    l.dw_splits = clip(dw.splits, tiles(rows_k, least));
+    const TilePlan dx = plan_tiles(q.n, q.d, terms * classes_k, true, cus);
     l.dx_tile = q.n <= 32 ? 3 : q.n <= 64 ? 2 : dx.big ? 0 : 1;
-    l.dx_splits = clip(dx.splits, tiles(l.piece * element, 128));
-    if (l.dx_splits * l.pieces > 1) l.dx_part = take(l.dx_splits * q.n * q.d * 4);
+    l.dx_splits = clip(dx.splits, tiles(classes_k, least));
+    const int64_t dw_bytes = l.dw_splits > 1 ? l.dw_splits * l.piece * q.d * 4 : 0;
+    const int64_t dx_bytes = l.dx_splits * l.pieces > 1 ? l.dx_splits * q.n * q.d * 4 : 0;
+    // (of one piece, dw's parts are joined before dX's are written)
+    if (l.pieces == 1) {
+      l.dw_part = l.dx_part = take(dw_bytes > dx_bytes ? dw_bytes : dx_bytes);
+    } else {
+      l.dw_part = take(dw_bytes);
+      l.dx_part = take(dx_bytes);
+    }
     l.bias_part = take(tiles(q.n, kTileRows[l.tile]) * q.v * 4);
   }
   l.total = at;
@@ -818,7 +791,7 @@ int launch_gradient_of(const ClassArgs& g, int tile, hipStream_t s) {
 }
 template <bool BK>
 int launch_gradient(const ClassArgs& g, const ClassLayout& l, int tile, hipStream_t s) {
-  return l.planes > 1 ? launch_gradient_of<BK, MmaF16, 2>(g, tile, s)
+  return l.planes > 1 ? launch_gradient_of<BK, MmaBf16, 2>(g, tile, s)
          : l.whole    ? launch_gradient_of<BK, MmaF32, 1>(g, tile, s)
                       : launch_gradient_of<BK, MmaBf16, 0>(g, tile, s);
 }
@@ -836,59 +809,45 @@ int sum_rows(const void* parts, int n_parts, int64_t n, bool f32, void* out, hip
 }
 
 // The operands X and w, packed where they have to be; `labels`: rows of X that are
-// ignored are left out (NULL: none).  With `g`, xg is X as the product with r over
-// the rows takes it: in planes, a row of r is in units of its own, which its row
-// of X makes up for.
+// ignored are left out (NULL: none); g: whose unit is wanted besides, or NULL.
 int operands(const ClassProblem& q, const ClassLayout& l, unsigned char* ws,
              const int64_t* labels, int64_t ignore, const float* g, hipStream_t s, TileOperand* x,
-             TileOperand* w, TileOperand* xg) {
+             TileOperand* w) {
   const int64_t e = q.esize();
   *x = TileOperand{static_cast<const unsigned char*>(q.x), q.ldx * e, 0, q.n, q.d * e};
   *w = TileOperand{static_cast<const unsigned char*>(q.w), q.ldw * e, 0, q.v, q.d * e};
-  const PackJob jx{q.x, q.n, q.d, q.ldx, ws + l.xp, labels,
-                   l.planes > 1 ? reinterpret_cast<const float*>(ws + l.row_max) : nullptr,
-                   nullptr, 0, g ? 2 : 0, 1};
-  const PackJob jw{q.w, q.v, q.d, q.ldw, ws + l.wp, nullptr, nullptr, nullptr, 1, 1, 1};
-  PackJob jg = jx;
-  jg.dst = ws + l.xg;
-  jg.row_max = nullptr;
-  jg.row_g = g;
-  jg.part_g = 2;
-  jg.writes = 0;
-  const TileOperand px{ws + l.xp, l.pitch, l.x_plane, q.n, l.pitch};
-  const TileOperand pw{ws + l.wp, l.pitch, l.w_plane, q.v, l.pitch};
   PackArgs a{};
   a.pitch = l.pitch;
   a.ignore = ignore;
   a.part = reinterpret_cast<const float*>(ws + l.maxima);
-  a.scale = reinterpret_cast<int*>(ws + l.scales);
-  a.row_max = reinterpret_cast<float*>(ws + l.row_max);
+  a.unit = reinterpret_cast<int*>(ws + l.units);
+  a.has_g = g != nullptr;
   int jobs = 0;
   int64_t most = 0;
   auto add = [&](const PackJob& j) {
     a.job[jobs++] = j;
     if (j.rows > most) most = j.rows;
   };
-  if (l.pack_x) add(jx), *x = px;
-  if (l.pack_w) add(jw), *w = pw;
-  if (xg) *xg = *x;
-  if (l.planes > 1) {                      // (both are packed)
-    if (xg) {
-      add(jg);
-      xg->base = ws + l.xg;
-    }
-    hipLaunchKernelGGL(part_max_kernel, dim3(kMaxParts, 3), dim3(256), 0, s, a, g,
-                       reinterpret_cast<float*>(ws + l.maxima));
-    ZS_LAUNCH_CHECK("part_max_kernel launch");
+  if (l.pack_x) {
+    add({q.x, q.n, q.d, q.ldx, ws + l.xp, labels});
+    *x = TileOperand{ws + l.xp, l.pitch, l.x_plane, q.n, l.pitch};
+  }
+  if (l.pack_w) {
+    add({q.w, q.v, q.d, q.ldw, ws + l.wp, nullptr});
+    *w = TileOperand{ws + l.wp, l.pitch, l.w_plane, q.v, l.pitch};
   }
   if (!jobs) return ZSHMC_OK;
   const dim3 grid(grid_for(most * (l.pitch / 16)), (unsigned)jobs);
-  if (l.planes > 1)
+  if (l.planes > 1) {                      // (both are packed)
+    hipLaunchKernelGGL(part_max_kernel, dim3(kMaxParts, 3), dim3(256), 0, s, a, g,
+                       reinterpret_cast<float*>(ws + l.maxima));
+    ZS_LAUNCH_CHECK("part_max_kernel launch");
     hipLaunchKernelGGL((pack_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
-  else if (q.f32())
+  } else if (q.f32()) {
     hipLaunchKernelGGL((pack_rows_kernel<float, false>), grid, dim3(256), 0, s, a);
-  else
+  } else {
     hipLaunchKernelGGL((pack_rows_kernel<uint16_t, false>), grid, dim3(256), 0, s, a);
+  }
   ZS_LAUNCH_CHECK("pack_rows_kernel launch");
   return ZSHMC_OK;
 }
@@ -959,15 +918,14 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   ClassArgs a{};
   a.part = reinterpret_cast<cf2*>(ws + l.part);
   a.label_logit = reinterpret_cast<float*>(ws + l.label_logit);
-  rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, nullptr, s, &a.b, &a.a,
-                nullptr);
+  rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, nullptr, s, &a.b, &a.a);
   if (rc != ZSHMC_OK) return rc;
   a.m = q.v;
   a.n = q.n;
   a.steps = (int)tiles(q.d * (l.whole ? 4 : 2), 128);
   a.terms = l.planes > 1 ? kTermsSplit : 1;
-  a.scale_m = reinterpret_cast<const int*>(ws + l.scales) + 1;
-  a.row_x = reinterpret_cast<const float*>(ws + l.row_max);
+  a.unit_b = reinterpret_cast<const int*>(ws + l.units);
+  a.unit_a = a.unit_b + 1;
   a.splits = 1;
   a.bias = bias;
   a.labels = labels;
@@ -977,9 +935,7 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
     a.out = ws + l.split_part;
     a.out_ld = q.v;
     a.out_split = q.n * q.v;
-    a.g = a.row_x;                 // (the rows' units)
-    a.row_units = 1;
-    rc = l.planes > 1 ? launch_tile<Few<MmaF16, 1>, kEpiStore, 2>(a, s)
+    rc = l.planes > 1 ? launch_tile<Few<MmaBf16, 1>, kEpiStore, 2>(a, s)
          : l.whole    ? launch_tile<Few<MmaF32, 1>, kEpiStore, 1>(a, s)
                       : launch_tile<Few<MmaBf16, 1>, kEpiStore, 0>(a, s);
     if (rc != ZSHMC_OK) return rc;
@@ -989,7 +945,7 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
     ZS_LAUNCH_CHECK("part_stats_kernel launch");
     return join_stats(q, l, a, labels, has_ignore, ignore_label, log_prob, stats, s);
   }
-  rc = l.planes > 1 ? launch_logits<MmaF16, kEpiStats, 2>(a, l.tile, s)
+  rc = l.planes > 1 ? launch_logits<MmaBf16, kEpiStats, 2>(a, l.tile, s)
        : l.whole    ? launch_logits<MmaF32, kEpiStats, 1>(a, l.tile, s)
                     : launch_logits<MmaBf16, kEpiStats, 0>(a, l.tile, s);
   if (rc != ZSHMC_OK) return rc;
@@ -1025,13 +981,13 @@ extern "C" int zshmc_class_log_prob_grad(
              "zshmc_class_log_prob_grad: %lld bytes of 16-byte aligned workspace needed, got "
              "%lld", (long long)l.total, (long long)workspace_bytes);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  TileOperand ox, ow, og;
+  TileOperand ox, ow;
   rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, grad_log_prob, s, &ox,
-                &ow, &og);
+                &ow);
   if (rc != ZSHMC_OK) return rc;
   const int terms = l.planes > 1 ? kTermsSplit : 1;
   const int64_t pb = l.whole ? 4 : 2;            // bytes of a plane's element
-  const int* scales = reinterpret_cast<const int*>(ws + l.scales);
+  const int* const unit = reinterpret_cast<const int*>(ws + l.units);    // of X, w, g
   const bool dx_joined = l.dx_splits * l.pieces > 1;
   for (int64_t c0 = 0; c0 < q.v; c0 += l.piece) {
     const int64_t c = q.v - c0 < l.piece ? q.v - c0 : l.piece;
@@ -1046,8 +1002,9 @@ extern "C" int zshmc_class_log_prob_grad(
     a.n = q.n;
     a.steps = (int)tiles(q.d * pb, 128);
     a.terms = terms;
-    a.scale_m = scales + 1;
-    a.row_x = reinterpret_cast<const float*>(ws + l.row_max);
+    a.unit_a = unit + 1;
+    a.unit_b = unit;
+    a.unit_g = unit + 2;
     a.splits = 1;
     a.bias = bias ? bias + c0 : nullptr;
     a.labels = labels;
@@ -1062,20 +1019,20 @@ extern "C" int zshmc_class_log_prob_grad(
     a.resid_plane = l.resid_plane;
     a.bias_part = grad_bias ? reinterpret_cast<float*>(ws + l.bias_part) : nullptr;
     a.bias_ld = q.v;
-    rc = l.planes > 1 ? launch_logits<MmaF16, kEpiResidual, 2>(a, l.tile, s)
+    rc = l.planes > 1 ? launch_logits<MmaBf16, kEpiResidual, 2>(a, l.tile, s)
          : l.whole    ? launch_logits<MmaF32, kEpiResidual, 1>(a, l.tile, s)
                       : launch_logits<MmaBf16, kEpiResidual, 0>(a, l.tile, s);
     if (rc != ZSHMC_OK) return rc;
     if (grad_w) {                  // dw = r^T X over the rows of X
       ClassArgs g{};
-      g.a = og;
+      g.a = ox;
       g.b = r;
       g.m = q.d;
       g.n = c;
       g.steps = (int)tiles(q.n * pb, 128);
       g.terms = terms;
-      g.scale_m = scales;
-      g.scale_n = scales + 2;
+      g.unit_a = unit;
+      g.unit_b = unit + 2;
       g.splits = l.dw_splits;
       g.out_ld = q.d;
       void* const dw = static_cast<unsigned char*>(grad_w) + c0 * q.d * q.esize();
@@ -1099,9 +1056,8 @@ extern "C" int zshmc_class_log_prob_grad(
       g.n = q.n;
       g.steps = (int)tiles(c * pb, 128);
       g.terms = terms;
-      g.scale_m = scales + 1;
-      g.g = grad_log_prob;
-      g.row_units = 1;
+      g.unit_a = unit + 1;
+      g.unit_b = unit + 2;
       g.splits = l.dx_splits;
       g.out_ld = q.d;
       if (dx_joined) {

@@ -310,7 +310,7 @@ __global__ __launch_bounds__(256, C::kLds > 80 * 1024 ? 1 : 2) void int8_tile_ke
     for (int r = 0; r < 4; ++r)
       v[r] = (float)acc_get(acc[i][j], 4 * q + r) * (sx[j] * sw[i][q][r]) + bias[i][q][r];
   };
-  tile_rows<C, As>(smem, lane, wave, value, [&](int, int n, int m, const tu4& piece) {
+  tile_rows<C, As>(smem, lane, wave, value, [&](int n, int m, const tu4& piece) {
     if (n0 + n < p.n && m0 + m < p.m)
       store_piece(static_cast<T*>(p.out) + (n0 + n) * p.ldo + m0 + m, p.m - m0 - m, piece);
   });

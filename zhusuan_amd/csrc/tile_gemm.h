@@ -32,11 +32,12 @@
 // 1385; eight waves of 128 x 64 each 1345, 64-byte steps in four buffers 1280,
 // two workgroups of 128 x 128 a CU 1105.
 //
-// `terms`: float32 operands may come as two float16 planes of x / 2^e, hi and lo =
-// the rest (22 bits and a sign; 2^e an operand's own, its largest magnitude near
-// 2^14, so that what float16 cannot hold is 2^-38 of that), and a product is hi lo
-// + lo hi + hi hi: what is left out is 2^-22 of it.  The loop runs over the pairs,
-// smallest first, into the same float32 accumulators.  One pair otherwise.
+// `terms`: float32 operands may come as three bfloat16 planes of x / 2^e: the nearest
+// one, the nearest to what it leaves, and the rest, 24 bits in all.  A product is the six
+// of nine plane products that are not below 2^-25 of it.  2^e is an operand's own, its
+// largest magnitude near 2^48, so that a product of 2^28 terms stays inside float32 and
+// all 24 bits of what is 2^-158 of the largest are still there.  The loop runs over the
+// pairs, smallest first, into the same float32 accumulators.  One pair otherwise.
 #pragma once
 #include <type_traits>
 #include <utility>
@@ -53,7 +54,6 @@ typedef float tf4 __attribute__((ext_vector_type(4)));
 typedef float tf16 __attribute__((ext_vector_type(16)));
 typedef int ti16 __attribute__((ext_vector_type(16)));
 typedef __bf16 tb8 __attribute__((ext_vector_type(8)));
-typedef _Float16 th8 __attribute__((ext_vector_type(8)));
 #define ZS_TLDS __attribute__((address_space(3)))
 
 // One operand as it lies in memory: rows x row_bytes, `pitch` bytes apart
@@ -64,10 +64,11 @@ struct TileOperand {
   int64_t rows, row_bytes;
 };
 
-// plane pairs, two bits each, smallest products first (one term: pair 0 0)
-constexpr int kTermsSplit = 3;
-constexpr uint32_t kTermsA = 0u | 1u << 2 | 0u << 4;
-constexpr uint32_t kTermsB = 1u | 0u << 2 | 0u << 4;
+// plane pairs, two bits each, smallest products first (one term: pair 0 0):
+// 1 1, 2 0, 0 2, 1 0, 0 1, 0 0
+constexpr int kPlanes = 3, kTermsSplit = 6;
+constexpr uint32_t kTermsA = 1u | 2u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+constexpr uint32_t kTermsB = 1u | 0u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
 
 // two float32 -> bfloat16 (to nearest even) in one register
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
@@ -76,15 +77,19 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   return __builtin_bit_cast(uint32_t, p);
 }
 
-__device__ __forceinline__ uint32_t f16_pair(float a, float b) {
-  typedef _Float16 pair __attribute__((ext_vector_type(2)));
-  const pair p = {(_Float16)a, (_Float16)b};
-  return __builtin_bit_cast(uint32_t, p);
-}
-// what float16 leaves of x (nothing of an infinity)
-__device__ __forceinline__ float f16_rest(float x) {
-  const float h = (float)(_Float16)x;
+// what bfloat16 leaves of x (nothing of an infinity)
+__device__ __forceinline__ float bf16_rest(float x) {
+  const float h = (float)(__bf16)x;
   return fabsf(h) == __builtin_inff() ? 0.f : x - h;
+}
+// the planes of two values
+__device__ __forceinline__ void bf16_planes(float a, float b, uint32_t (&plane)[kPlanes]) {
+#pragma unroll
+  for (int k = 0; k < kPlanes; ++k) {
+    plane[k] = bf16_pair(a, b);
+    a = bf16_rest(a);
+    b = bf16_rest(b);
+  }
 }
 
 // kBytes: of an element of a k-major operand
@@ -94,14 +99,6 @@ struct MmaBf16 {
   static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
         __builtin_bit_cast(tb8, a), __builtin_bit_cast(tb8, b), c, 0, 0, 0);
-  }
-};
-struct MmaF16 {
-  typedef tf16 Acc;
-  static constexpr int kBytes = 2;
-  static __device__ __forceinline__ Acc mma(const tu4& a, const tu4& b, const Acc& c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
-        __builtin_bit_cast(th8, a), __builtin_bit_cast(th8, b), c, 0, 0, 0);
   }
 };
 // float32 as it is: a lane's four elements of a chunk one MFMA each (k is a dummy
@@ -491,35 +488,23 @@ __device__ __forceinline__ int acc_get(const ti16& v, int r) {
 // WGN x 32 rows of BM values are written as elements T (float, or bfloat16 bits),
 // 16 bytes between rows so that they start in different banks, and read back
 // in 16-byte pieces; two regions alternate, one barrier a block column.
-// As: how a value is written (AsF32, AsBf16, or AsF16Planes: two rows, what float16
-// holds of it and the rest).
+// As: how a value is written (AsF32, AsBf16).
 //   value(i, j, q, v): the four values of registers 4 q .. 4 q + 3 of block (i, j)
-//   emit(plane, n, m, piece): 16 bytes of row n (of the tile) from column m on
+//   emit(n, m, piece): 16 bytes of row n (of the tile) from column m on
 struct AsF32 {
   typedef float T;
-  static constexpr int kPlanes = 1;
-  static __device__ __forceinline__ void put(char* to, int, const float (&v)[4]) {
+  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
     *reinterpret_cast<tf4*>(to) = tf4{v[0], v[1], v[2], v[3]};
   }
 };
 struct AsBf16 {
   typedef uint16_t T;
-  static constexpr int kPlanes = 1;
-  static __device__ __forceinline__ void put(char* to, int, const float (&v)[4]) {
+  static __device__ __forceinline__ void put(char* to, const float (&v)[4]) {
     *reinterpret_cast<tu2*>(to) = tu2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
   }
 };
-struct AsF16Planes {
-  typedef uint16_t T;
-  static constexpr int kPlanes = 2;
-  static __device__ __forceinline__ void put(char* to, int plane, const float (&v)[4]) {
-    *reinterpret_cast<tu2*>(to) = tu2{f16_pair(v[0], v[1]), f16_pair(v[2], v[3])};
-    *reinterpret_cast<tu2*>(to + plane) = tu2{f16_pair(f16_rest(v[0]), f16_rest(v[1])),
-                                              f16_pair(f16_rest(v[2]), f16_rest(v[3]))};
-  }
-};
 template <typename C, typename As>
-constexpr int kTileRowsLds = 2 * As::kPlanes * C::WGN * 32 * (C::BM * (int)sizeof(typename As::T) + 16);
+constexpr int kTileRowsLds = 2 * C::WGN * 32 * (C::BM * (int)sizeof(typename As::T) + 16);
 
 template <typename C, typename As, typename V, typename E>
 __device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& value, E&& emit) {
@@ -531,26 +516,22 @@ __device__ __forceinline__ void tile_rows(char* smem, int lane, int wave, V&& va
                      ((wave / C::WGN) * C::WM * 32 + 4 * half) * (int)sizeof(T);
   tile_for<C::WN>([&](auto J) {
     constexpr int j = decltype(J)::value;
-    constexpr int region = (j & 1) * As::kPlanes * kRows * kPitch;
+    constexpr int region = (j & 1) * kRows * kPitch;
     tile_for<C::WM>([&](auto I) {
       constexpr int i = decltype(I)::value;
       tile_for<4>([&](auto Q) {
         constexpr int q = decltype(Q)::value;
         float v[4];
         value(I, J, Q, v);
-        As::put(mine + region + (i * 32 + 8 * q) * (int)sizeof(T), kRows * kPitch, v);
+        As::put(mine + region + (i * 32 + 8 * q) * (int)sizeof(T), v);
       });
     });
     __syncthreads();
-    tile_for<As::kPlanes>([&](auto P) {
-      constexpr int plane = decltype(P)::value;
-      for (int c = threadIdx.x; c < kRows * kPieces; c += 256) {
-        const int row = c / kPieces, piece = c % kPieces;
-        emit(plane, (row >> 5) * C::WN * 32 + j * 32 + (row & 31), piece * kPer,
-             *reinterpret_cast<const tu4*>(smem + region + plane * kRows * kPitch +
-                                           row * kPitch + piece * 16));
-      }
-    });
+    for (int c = threadIdx.x; c < kRows * kPieces; c += 256) {
+      const int row = c / kPieces, piece = c % kPieces;
+      emit((row >> 5) * C::WN * 32 + j * 32 + (row & 31), piece * kPer,
+           *reinterpret_cast<const tu4*>(smem + region + row * kPitch + piece * 16));
+    }
   });
 }
 

@@ -460,12 +460,17 @@ class LinearClassLogits(object):
     w may also be the 8-bit rows [K, F] that `quantize_rows` returns: a model
     that is done learning answers from them (`quantized_linear`, no gradient)."""
 
-    # From how many logits a chain, and classes, log_prob takes the classes in
-    # pieces rather than writing the logits out: float32, 1024 x 784, log_prob
-    # with its gradient over 4096 classes (2^22) 146 us against 221, over 512
-    # (2^19) 145 against 178 of a host's time either way; 8192 x 2048 over 512
-    # classes 340 against 267, over 4096 1270 against 2010.
-    MANY_LOGITS, MANY_CLASSES = 1 << 22, 1024
+    # From how many logits a chain, and how many classes (a feature, too),
+    # log_prob takes the classes in pieces rather than writing the logits out.
+    # float32 log_prob with w's gradient in pieces / written out, us, by rows x
+    # features x classes: 1024 x 256 x 4096 110 / 124, 1024 x 784 x 4096 222 /
+    # 228, 8192 x 784 x 4096 958 / 1061, 2000 x 300 x 20 000 593 / 1078; fewer
+    # classes a feature 1024 x 1024 x 4096 242 / 214, 300 x 4096 x 14 000 1280 /
+    # 832; fewer classes 4096 x 256 x 1024 110 / 71.  From MOST_LOGITS of all
+    # chains on (8 GB an array, and there are three) memory decides.  A
+    # program that wants one or the other sets them on its own object.
+    MANY_LOGITS, MANY_CLASSES, CLASSES_A_FEATURE = 1 << 22, 1024, 5
+    MOST_LOGITS = 1 << 31
 
     def __init__(self, w, X):
         if not isinstance(w, _ops.QuantizedRows):
@@ -516,9 +521,16 @@ class LinearClassLogits(object):
                 not self.X.requires_grad and self.dtype == torch.float32)
 
     def many_ok(self):
+        n = self.n_rows * self.n_classes
+        chains = 1
+        for d in self.lead_shape:
+            chains *= int(d)
         return (not self.quantized and
-                self.n_classes >= self.MANY_CLASSES and
-                self.n_rows * self.n_classes >= self.MANY_LOGITS and
+                ((self.n_classes >= max(
+                    self.MANY_CLASSES,
+                    self.CLASSES_A_FEATURE * self.n_features) and
+                  n >= self.MANY_LOGITS) or
+                 chains * n >= self.MOST_LOGITS) and
                 self.dtype == torch.float32 and
                 self.X.dtype == torch.float32 and
                 self.w.device == self.X.device and self.w.is_cuda)

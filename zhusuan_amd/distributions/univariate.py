@@ -520,17 +520,22 @@ class LinearClassLogits(object):
                 self.n_features <= _ops.MAX_LIKELIHOOD_WIDTH and
                 not self.X.requires_grad and self.dtype == torch.float32)
 
-    def many_ok(self):
+    def many_classes(self):
+        """Are these sizes taken in pieces?  (Sizes that the pieces' entry
+        point does not take are not.)"""
         n = self.n_rows * self.n_classes
         chains = 1
         for d in self.lead_shape:
             chains *= int(d)
-        return (not self.quantized and
-                ((self.n_classes >= max(
-                    self.MANY_CLASSES,
-                    self.CLASSES_A_FEATURE * self.n_features) and
-                  n >= self.MANY_LOGITS) or
+        return (self.n_classes >= self.MANY_CLASSES and
+                n >= self.MANY_LOGITS and
+                (self.n_classes >= self.CLASSES_A_FEATURE * self.n_features or
                  chains * n >= self.MOST_LOGITS) and
+                chains > 0 and 0 < self.n_features <= 1 << 20 and
+                self.n_rows < 1 << 28 and self.n_classes < 1 << 31)
+
+    def many_ok(self):
+        return (not self.quantized and self.many_classes() and
                 self.dtype == torch.float32 and
                 self.X.dtype == torch.float32 and
                 self.w.device == self.X.device and self.w.is_cuda)

@@ -1033,6 +1033,8 @@ int zshmc_uni2_sample(int kind, float* out, const float* a, const float* b,
  *                  gradients only where grad_log_prob is not 0
  *   stats          [n_rows][2] float32 (maximum, sum of exponentials) for the
  *                  gradient, 8-byte aligned, or NULL
+ *   sizes          at most 2^27 rows, 2^31 - 1 classes, 2^20 features, and fewer
+ *                  than 2^24 tiles of 128 or 256 rows x classes
  *   workspace      16-byte aligned; its size from
  *                  zshmc_class_log_prob_workspace with the SAME pointers and
  *                  strides (gradient = 0 / 1 for the two calls), written to

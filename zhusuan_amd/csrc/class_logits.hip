@@ -758,7 +758,7 @@ int launch_tile(const ClassArgs& a, hipStream_t s) {
   p.tiles_m = (uint32_t)tiles(p.m, C::BM);
   p.tiles_n = (uint32_t)tiles(p.n, C::BN);
   const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n;
-  ZS_REQUIRE(wgs < (1ll << 31), "class logits: %lld tiles", (long long)wgs);
+  ZS_REQUIRE(wgs <= kMaxWorkgroups, "class logits: %lld tiles", (long long)wgs);
   hipLaunchKernelGGL((class_tile_kernel<C, EPI, F32>), dim3((unsigned)wgs, (unsigned)p.splits),
                      dim3(256), lds, s, p);
   ZS_LAUNCH_CHECK("class_tile_kernel launch");
@@ -874,9 +874,23 @@ int check_problem(const ClassProblem& q, const char* who) {
              "%s: dtype must be ZSHMC_DTYPE_F32 or _BF16, got %d", who, q.dtype);
   ZS_REQUIRE(q.n >= 0 && q.d > 0 && q.v > 0, "%s: n_rows >= 0, n_features and n_classes > 0",
              who);
-  ZS_REQUIRE(q.n < (1ll << 31) && q.v < (1ll << 31) && q.d <= (1ll << 20),
-             "%s: at most 2^31 - 1 rows and classes and 2^20 features", who);
+  ZS_REQUIRE(q.n <= (1ll << 27) && q.v < (1ll << 31) && q.d <= (1ll << 20),
+             "%s: at most 2^27 rows, 2^31 - 1 classes and 2^20 features", who);
   ZS_REQUIRE(q.ldx >= q.d && q.ldw >= q.d, "%s: rows overlap (ldx / ldw < n_features)", who);
+  return ZSHMC_OK;
+}
+
+// every launch of a call within what HIP launches, in front of the first one
+int check_tiles(const ClassProblem& q, const ClassLayout& l, bool grad, const char* who) {
+  int64_t most = tiles(l.piece, kTileClasses[l.tile]) * tiles(q.n, kTileRows[l.tile]);
+  if (grad) {
+    const int64_t b = l.dw_tile ? 128 : 256, dw = tiles(q.d, b) * tiles(l.piece, b);
+    const int64_t dx = tiles(q.d, l.dx_tile ? 128 : 256) * tiles(q.n, kTileRows[l.dx_tile]);
+    most = most > dw ? most : dw;
+    most = most > dx ? most : dx;
+  }
+  ZS_REQUIRE(most <= kMaxWorkgroups, "%s: %lld tiles, more than one launch takes", who,
+             (long long)most);
   return ZSHMC_OK;
 }
 
@@ -913,6 +927,8 @@ extern "C" int zshmc_class_log_prob(const void* x, const void* w, const float* b
   ZS_REQUIRE(workspace_bytes >= l.total && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "zshmc_class_log_prob: %lld bytes of 16-byte aligned workspace needed, got %lld",
              (long long)l.total, (long long)workspace_bytes);
+  rc = check_tiles(q, l, false, "zshmc_class_log_prob");
+  if (rc != ZSHMC_OK) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   ClassArgs a{};
@@ -980,6 +996,8 @@ extern "C" int zshmc_class_log_prob_grad(
   ZS_REQUIRE(workspace_bytes >= l.total && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "zshmc_class_log_prob_grad: %lld bytes of 16-byte aligned workspace needed, got "
              "%lld", (long long)l.total, (long long)workspace_bytes);
+  rc = check_tiles(q, l, true, "zshmc_class_log_prob_grad");
+  if (rc != ZSHMC_OK) return rc;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   TileOperand ox, ow;
   rc = operands(q, l, ws, has_ignore ? labels : nullptr, ignore_label, grad_log_prob, s, &ox,

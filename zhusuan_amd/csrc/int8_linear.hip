@@ -322,6 +322,12 @@ int launch_int8(const Int8Args& a, hipStream_t s) {
       kTileRowsLds<C, typename std::conditional<BF16, AsBf16, AsF32>::type> + C::BM * 8;
   constexpr int lds = C::kLds > epi ? C::kLds : epi;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
+  Int8Args p = a;
+  p.tiles_m = (uint32_t)((p.m + C::BM - 1) / C::BM);
+  p.tiles_n = (uint32_t)((p.n + C::BN - 1) / C::BN);
+  const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n;
+  ZS_REQUIRE(wgs <= kMaxWorkgroups, "zshmc_int8_linear: %lld tiles, more than one launch takes",
+             (long long)wgs);
   static thread_local int attr_dev = -1;
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
@@ -332,11 +338,6 @@ int launch_int8(const Int8Args& a, hipStream_t s) {
     if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(LDS)");
     attr_dev = dev;
   }
-  Int8Args p = a;
-  p.tiles_m = (uint32_t)((p.m + C::BM - 1) / C::BM);
-  p.tiles_n = (uint32_t)((p.n + C::BN - 1) / C::BN);
-  const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n;
-  ZS_REQUIRE(wgs < (1ll << 31), "zshmc_int8_linear: %lld tiles", (long long)wgs);
   hipLaunchKernelGGL((int8_tile_kernel<C, BF16>), dim3((unsigned)wgs), dim3(256), lds, s, p);
   ZS_LAUNCH_CHECK("int8_tile_kernel launch");
   return ZSHMC_OK;
@@ -361,25 +362,28 @@ int launch_quantize(const void* x, int64_t n_rows, int64_t n_cols, int64_t ldx, 
                     int8_t* values, int64_t pitch, float* scale, hipStream_t s) {
   // a wave per row where that is eight waves a CU or more
   const bool wave = n_rows >= 8ll * device_cu_count();
-  const unsigned grid = (unsigned)(wave ? (n_rows + 3) / 4 : n_rows);
-  if (dtype == ZSHMC_DTYPE_F32) {
-    const float* f = static_cast<const float*>(x);
-    if (wave)
-      hipLaunchKernelGGL((quantize_rows_kernel<float, 64>), dim3(grid), dim3(256), 0, s, f, n_rows,
-                         (int)n_cols, ldx, values, (int)pitch, scale);
+  // (in launches of at most 2^25 rows, see kMaxWorkgroups)
+  constexpr int64_t kRows = 1ll << 25;
+  for (int64_t r = 0; r < n_rows; r += kRows) {
+    const int64_t rows = n_rows - r < kRows ? n_rows - r : kRows;
+    const unsigned grid = (unsigned)(wave ? (rows + 3) / 4 : rows);
+    auto launch = [&](auto* f) {
+      typedef typename std::remove_cv<typename std::remove_pointer<decltype(f)>::type>::type T;
+      if (wave)
+        hipLaunchKernelGGL((quantize_rows_kernel<T, 64>), dim3(grid), dim3(256), 0, s,
+                           f + r * ldx, rows, (int)n_cols, ldx, values + r * pitch, (int)pitch,
+                           scale + r);
+      else
+        hipLaunchKernelGGL((quantize_rows_kernel<T, 256>), dim3(grid), dim3(256), 0, s,
+                           f + r * ldx, rows, (int)n_cols, ldx, values + r * pitch, (int)pitch,
+                           scale + r);
+    };
+    if (dtype == ZSHMC_DTYPE_F32)
+      launch(static_cast<const float*>(x));
     else
-      hipLaunchKernelGGL((quantize_rows_kernel<float, 256>), dim3(grid), dim3(256), 0, s, f,
-                         n_rows, (int)n_cols, ldx, values, (int)pitch, scale);
-  } else {
-    const uint16_t* f = static_cast<const uint16_t*>(x);
-    if (wave)
-      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, 64>), dim3(grid), dim3(256), 0, s, f,
-                         n_rows, (int)n_cols, ldx, values, (int)pitch, scale);
-    else
-      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, 256>), dim3(grid), dim3(256), 0, s, f,
-                         n_rows, (int)n_cols, ldx, values, (int)pitch, scale);
+      launch(static_cast<const uint16_t*>(x));
+    ZS_LAUNCH_CHECK("quantize_rows_kernel launch");
   }
-  ZS_LAUNCH_CHECK("quantize_rows_kernel launch");
   return ZSHMC_OK;
 }
 

@@ -425,6 +425,9 @@ __device__ __forceinline__ void tile_of_block(uint32_t bid, uint32_t n_wg, uint3
   tn = __builtin_amdgcn_readfirstlane((int)c);
 }
 
+// HIP launches fewer than 2^32 threads along a dimension of the grid
+constexpr int64_t kMaxWorkgroups = (1ll << 24) - 1;
+
 // 256 x 256 tiles (one workgroup a CU) or 128 x 128 (two)?  And, for a product whose
 // k may be split with the parts joined afterwards, over how many workgroups?  What
 // takes the fewest of a large tile's steps (1.6 us): a CU's two small tiles take 0.58

@@ -532,7 +532,7 @@ class LinearClassLogits(object):
                 (self.n_classes >= self.CLASSES_A_FEATURE * self.n_features or
                  chains * n >= self.MOST_LOGITS) and
                 chains > 0 and 0 < self.n_features <= 1 << 20 and
-                self.n_rows < 1 << 28 and self.n_classes < 1 << 31)
+                self.n_rows <= 1 << 27 and self.n_classes < 1 << 31)
 
     def many_ok(self):
         return (not self.quantized and self.many_classes() and

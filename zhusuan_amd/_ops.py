@@ -1267,14 +1267,15 @@ class QuantizedRows(object):
 
     @staticmethod
     def _usable(rows):
-        """Rows of whole 16 bytes, readable to their end."""
+        """Rows of whole 16 bytes, readable to their end, at a pitch that the
+        product takes."""
         n, K = rows.shape
         if n == 0:
             return False
         pitch = rows.stride(0) if n > 1 else (K + 15) // 16 * 16
         end = rows.storage_offset() + (n - 1) * pitch + (K + 15) // 16 * 16
         return ((K == 1 or rows.stride(1) == 1) and pitch % 16 == 0 and
-                pitch >= (K + 15) // 16 * 16 and
+                (K + 15) // 16 * 16 <= pitch <= 4 << 20 and
                 rows.data_ptr() % 16 == 0 and
                 end <= rows.untyped_storage().nbytes())
 

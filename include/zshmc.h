@@ -1077,7 +1077,8 @@ int zshmc_dequantize_rows(const int8_t* values, int64_t pitch,
                           const float* scale, int64_t n_rows, int64_t n_cols,
                           void* out, int64_t ldo, int dtype, void* stream);
 /* out[m, n] = (x_scale[m] w_scale[n]) sum_k x[m, k] w[n, k] + bias[n] with
- * 8-bit x and w and an exact sum (n_features <= 131072); bias may be NULL.
+ * 8-bit x and w and an exact sum (n_features <= 131072, where x and w do not
+ * both hold -128: 131072 products of it are 2^31); bias may be NULL.
  * Rows are 16-byte aligned with pitches of whole 16 bytes and readable up to
  * the next multiple of 16 columns, where x holds zeros. */
 int zshmc_int8_linear(const int8_t* x, int64_t x_pitch, const float* x_scale,

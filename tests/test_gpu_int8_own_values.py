@@ -1,4 +1,4 @@
-"""8-bit values that a program brings: rows further apart
+"""8-bit values that a program brings: the smallest one, and rows further apart
 than the product's kernels take."""
 import pytest
 import torch
@@ -6,6 +6,32 @@ import torch
 import zhusuan_amd as zs
 
 pytestmark = pytest.mark.gpu
+
+
+def lowest(rows, K):
+    return zs.QuantizedRows(torch.full((rows, K), -128, dtype=torch.int8,
+                                       device='cuda'),
+                            torch.ones(rows, device='cuda'))
+
+
+def test_products_of_the_lowest_value():
+    """K products of 2^14 are exact up to K = 131071, and refused where their
+    sum, 2^31, is no int32."""
+    K = 131071
+    got = zs.quantized_linear(lowest(3, K), lowest(2, K))
+    assert torch.equal(got, torch.full_like(got, float(K * 2 ** 14)))
+    with pytest.raises(ValueError, match='131071'):
+        zs.quantized_linear(lowest(3, K + 1), lowest(2, K + 1))
+    # one side rounded here stays within 127 * 128
+    one = torch.ones(2, K + 1, device='cuda')
+    for X in (one, zs.quantize_rows(one)):
+        got = zs.quantized_linear(lowest(3, K + 1), X) * 127
+        ref = torch.full_like(got, -127. * 128 * (K + 1))
+        # (1 / 127 as the scale, and two products with it)
+        assert bool(((got - ref).abs() <= 4 * 2.0 ** -24 * ref.abs()).all())
+    got = zs.quantized_linear(zs.quantize_rows(one), lowest(3, K + 1)) * 127
+    assert bool(((got + 127. * 128 * (K + 1)).abs() <=
+                 4 * 2.0 ** -24 * 127. * 128 * (K + 1)).all())
 
 
 def test_rows_far_apart():

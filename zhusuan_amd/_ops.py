@@ -1224,7 +1224,8 @@ def linear_categorical_log_prob(w, X, labels, bias=None, ignore_label=None):
 class QuantizedRows(object):
     """A matrix [..., K] as 8-bit integers with one float32 scale per row,
     x ~ values * scale: what `quantize_rows` returns and `quantized_linear`
-    multiplies.  `values` int8 [..., K], `scale` float32 [...].  Values in
+    multiplies.  `values` int8 [..., K] (-128 too, which quantize_rows does not
+    make), `scale` float32 [...].  Values in
     rows of whole, aligned 16 bytes are used where they lie (a later write to
     them is seen); others are copied into such rows here, once."""
 
@@ -1250,8 +1251,9 @@ class QuantizedRows(object):
         # (zeros behind the last column, as the left operand needs them?)
         self._set(shape, rows, scale, K % 16 == 0)
 
-    def _set(self, shape, rows, scale, zero_tail):
+    def _set(self, shape, rows, scale, zero_tail, within_127=False):
         self._shape, self._rows, self.scale = shape, rows, scale
+        self._within_127 = within_127
         self._flat_scale = scale.reshape(-1).contiguous() \
             if scale.dim() != 1 or not scale.is_contiguous() else scale
         self._zero_tail = zero_tail
@@ -1262,7 +1264,7 @@ class QuantizedRows(object):
     def _of(cls, shape, rows, scale):
         """What quantize_rows has just written."""
         q = cls.__new__(cls)
-        q._set(shape, rows, scale.reshape(shape[:-1]), True)
+        q._set(shape, rows, scale.reshape(shape[:-1]), True, True)
         return q
 
     @staticmethod
@@ -1370,6 +1372,11 @@ def quantized_linear(w, X, bias=None, dtype=None):
     if K > 131072:
         raise ValueError("quantized_linear: at most 131072 columns (the sum "
                          "is an int32), got {}".format(K))
+    if K == 131072 and isinstance(X, QuantizedRows) and \
+            not (w._within_127 or X._within_127):
+        raise ValueError("quantized_linear: at most 131071 columns of values "
+                         "of one's own (131072 products of -128 pass an "
+                         "int32), got {}".format(K))
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or not \
                 bias.dtype.is_floating_point or tuple(bias.shape) != (V,):

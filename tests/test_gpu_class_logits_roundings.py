@@ -1,5 +1,5 @@
-"""float32 operands of zs.linear_categorical_log_prob are float32 to the last
-bit that a float32 evaluation has: rows, features and upstream gradients of
+"""What zs.linear_categorical_log_prob is off by, as independent roundings.  float32
+operands are float32 to the last bit that a float32 evaluation has: rows, features and upstream gradients of
 very different sizes, rare classes, infinite and extreme weights.
 
 helpers_class_logits bounds the worst case, K roundings of a sum of K terms all one
@@ -49,7 +49,9 @@ def plain(w, X, y, b, g, dtype):
 
 
 def spread(w, X, y, b, g):
-    """Variances of log_prob, dw, dX and db, see above."""
+    """Variances of log_prob, dw, dX and db, see above.  bfloat16 operands: r, dw
+    and dX are rounded to it, half a step, 2^-8, at most (db sums r before that)."""
+    half = 2.0 ** 32 if w.dtype == torch.bfloat16 else 0.
     w, X, g = w.double(), X.double(), g.double()[:, None]
     N, D = X.shape
     V = w.shape[0]
@@ -73,11 +75,12 @@ def spread(w, X, y, b, g):
     v_r = (g * p).square() * v_p + 4 * g * g * (hot + p * p)
     x2, w2, r2 = X * X, w * w, r * r
     dw, dx, db = r.t() @ X, r @ w, r.sum(0)
-    v_w = v_r.t() @ x2 + N / 4 * (r2.t() @ x2 + dw * dw) + dw * dw
-    # (a row's log-sum-exp is off for all of its classes alike)
-    v_x = v_r @ w2 + V / 4 * (r2 @ w2 + dx * dx) + dx * dx + \
-        v_lse * ((g * p) @ w).square()
     v_b = v_r.sum(0) + N / 4 * (r2.sum(0) + db * db) + db * db
+    v_r = v_r + half * r2
+    v_w = v_r.t() @ x2 + N / 4 * (r2.t() @ x2 + dw * dw) + (1 + half) * dw * dw
+    # (a row's log-sum-exp is off for all of its classes alike)
+    v_x = v_r @ w2 + V / 4 * (r2 @ w2 + dx * dx) + (1 + half) * dx * dx + \
+        v_lse * ((g * p) @ w).square()
     return [2.0 ** -48 * v for v in (v_lp[:, 0], v_w, v_x, v_b)]
 
 
@@ -100,6 +103,7 @@ def check(w, X, y, b, g, rows=False):
     as_good_as_float32(ours(w, X, y, b, g), w, X, y, b, g, rows)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('N,D,V', [
     (20, 96, 700),                   # 32 rows a tile
     (60, 96, 700),                   # 64
@@ -107,15 +111,16 @@ def check(w, X, y, b, g, rows=False):
     (81, 64, 300), (129, 72, 4099), (270, 100, 12419), (600, 130, 1000),
     (700, 256, 4000), (1021, 784, 1237), (2000, 300, 20000),
     (9001, 64, 15001)])              # pieces
-def test_no_part_of_a_product_is_lost(N, D, V):
+def test_no_part_of_a_product_is_lost(N, D, V, dtype):
     for bias in (False, True):
-        check(*problem(N, D, V, torch.float32, N + D, bias))
+        check(*problem(N, D, V, dtype, N + D, bias))
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('N,D,V', [(7, 2816, 1029), (300, 2500, 130),
                                    (700, 2048, 260)])
-def test_no_part_is_lost_of_many_features(N, D, V):
-    check(*problem(N, D, V, torch.float32, N + D, True))
+def test_no_part_is_lost_of_many_features(N, D, V, dtype):
+    check(*problem(N, D, V, dtype, N + D, True))
 
 
 @pytest.mark.parametrize('N', [60, 300, 900])
@@ -214,3 +219,75 @@ def test_through_a_categorical():
         zs.linear_class_logits(leaf, X)).log_prob(y.int())
     gw, = torch.autograd.grad(lp, leaf, g)
     as_good_as_float32([lp.detach(), gw], w, X, y, None, g)
+
+
+# Sums of one product each, in operands of 24 bits: a part of the product that is
+# lost, 2^-18 of it and more, cannot hide in the roundings of a long sum.
+ONE = [(20, 300), (60, 300), (129, 700), (300, 700), (600, 1000), (1021, 1237),
+       (2100, 20000)]
+
+
+def off(got, ref, rel, extra=0.):
+    bad = (got.double() - ref).abs() > rel * ref.abs() + extra
+    assert not bool(bad.any()), (int(bad.sum()), float(
+        ((got.double() - ref).abs() / ref.abs()).nan_to_num(0.).max()))
+
+
+def diagonal(N, dtype=torch.float32, seed=0):
+    """[N, N] with random values on the diagonal, and N random numbers."""
+    gen = torch.Generator().manual_seed(seed)
+    x = (0.5 + torch.rand(N, generator=gen)).to(dtype)
+    return torch.diag(x).cuda(), (0.5 + torch.rand(N, generator=gen)).cuda(), \
+        torch.randperm(1 << 20, generator=gen)[:N].cuda()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('N,V', ONE)
+def test_single_products_in_the_logits(N, V, dtype):
+    """Row n has one feature; its label's class a weight of about -1000 there,
+    the others 0, so that log_prob is that product less log(V - 1): a rounding
+    of the product, of its difference to 0 and of log_prob, at most 6 u with what
+    the planes leave out, and log(V - 1) < 16 from a sum that is exact."""
+    X, v, y = diagonal(N, dtype)
+    y = y % V
+    w = torch.zeros(V, N, device='cuda')
+    w[y, torch.arange(N, device='cuda')] = -1000 * v
+    w = w.to(dtype)
+    lp = zs.linear_categorical_log_prob(w, X, y)
+    l = X.diagonal().double() * w[y, torch.arange(N, device='cuda')].double()
+    ref = l - torch.log(V - 1 + l.exp())
+    off(lp, ref, 6 * 2.0 ** -24, 16 * 2.0 ** -23)
+
+
+@pytest.mark.parametrize('N,V', ONE)
+def test_single_products_in_the_gradient_of_w(N, V):
+    """w = 0: r = g ([v == y] - 1 / V), four roundings; dw has one product an
+    element, at most 2 u with what the planes leave out, and one rounding."""
+    X, g, y = diagonal(N, seed=1)
+    y = y % V
+    w = torch.zeros(V, N, device='cuda', requires_grad=True)
+    dw, = torch.autograd.grad(zs.linear_categorical_log_prob(w, X, y), w, g)
+    r = torch.full((N, V), -1. / V, dtype=torch.float64, device='cuda')
+    r[torch.arange(N, device='cuda'), y] += 1
+    off(dw, (r * (g.double() * X.diagonal().double())[:, None]).t(),
+        8 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize('N,V', ONE)
+def test_single_products_in_the_gradient_of_X(N, V):
+    """X = 0, and each feature has a weight in one class."""
+    gen = torch.Generator().manual_seed(2)
+    D = 200
+    at = torch.randperm(V, generator=gen)[:D].cuda()
+    w = torch.zeros(V, D, device='cuda')
+    w[at, torch.arange(D, device='cuda')] = (
+        0.5 + torch.rand(D, generator=gen)).cuda()
+    _, g, y = diagonal(N, seed=3)
+    y = y % V
+    X = torch.zeros(N, D, device='cuda', requires_grad=True)
+    dx, = torch.autograd.grad(zs.linear_categorical_log_prob(w, X, y), X, g)
+    r = torch.full((N, V), -1. / V, dtype=torch.float64, device='cuda')
+    r[torch.arange(N, device='cuda'), y] += 1
+    ref = g.double()[:, None] * r[:, at] * w[
+        at, torch.arange(D, device='cuda')].double()
+    off(dx, ref, 8 * 2.0 ** -24)

@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ZSHMC_VERSION 600 /* 0.6.0: + the documents' own vocabularies in the bf16x3 multinomial kernel (zshmc_linear_multinomial_log_lik_bf16x3_sparse, zshmc_model_plan.obs_sp_*); 0.5.1: packed rows, zshmc_bf16x3_multinomial_rows_packed; 0.5.0: the bf16x3 likelihood kernels, zshmc_model_plan.inner_image */
+#define ZSHMC_VERSION 600 /* 0.6.0 (the output layer's entry points at the end came later under the same number: nothing before them moved): + the documents' own vocabularies in the bf16x3 multinomial kernel (zshmc_linear_multinomial_log_lik_bf16x3_sparse, zshmc_model_plan.obs_sp_*); 0.5.1: packed rows, zshmc_bf16x3_multinomial_rows_packed; 0.5.0: the bf16x3 likelihood kernels, zshmc_model_plan.inner_image */
 
 /* status codes */
 #define ZSHMC_OK 0

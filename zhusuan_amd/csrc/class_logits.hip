@@ -683,16 +683,17 @@ ClassLayout layout_of(const ClassProblem& q, bool grad, bool has_ignore) {
            : q.n <= 64                                          ? 2
            : plan_tiles(l.piece, q.n, terms * tiles(q.d * element, 128), false, cus).big ? 0
                                                                                          : 1;
-  // (half the chip or more without a tile: halve them.  float32 1065 x 3456, 1122
-  // classes: 81 tiles 84 us, 153 halves 73; 128 x 2048, 4096 classes: 64 halves 82 us,
-  // 128 quarters 50)
+  // (half the chip or more without a tile: halve them.  Forward call, float32, 1065 x
+  // 3456, 1122 classes: 81 tiles 196 us, 153 halves 176; 128 x 2048, 4096 classes: 32
+  // tiles 139 us, 128 quarters 55)
   while (l.tile > 0 && l.tile < 3 &&
          tiles(l.piece, 128) * tiles(q.n, kTileRows[l.tile]) * 2 <= cus)
     ++l.tile;
   l.tiles_v = tiles(q.v, kTileClasses[l.tile]);
   // Still half the chip or more without one, and many features: logits of a share of
-  // the features a workgroup, in parts, which a pass of its own joins.  float32 7 x
-  // 2816 over 4945 classes (39 tiles): 66 us whole, 24 in 8 parts
+  // the features a workgroup, in parts, which a pass of its own joins.  Forward call,
+  // float32 7 x 2816 over 4945 classes (39 tiles): 70 us whole, 30 in 8 parts; 128 x
+  // 2048 over 4096: 55, 39 in 4; bfloat16, with half the steps: 24 and 22, 25 and 25
   l.splits = 1;
   l.split_part = 0;
   const int64_t all_tiles = l.tiles_v * tiles(q.n, kTileRows[l.tile]);

@@ -208,7 +208,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(
 }
 
 // Four values a thread, the row's scale beside them; bound by memory: 131 072 x 4096
-// to float32 504 us, 5.3 TB/s of 1 byte in and 4 out (a large copy: 4.9).
+// to float32 504 us, 5.3 TB/s of 1 byte in and 4 out (a large copy: 4.9); to bfloat16 317
+// us, 5.1.
 template <bool BF16>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(
     const int8_t* __restrict__ q, int64_t pitch, const float* __restrict__ scale, int64_t rows,

@@ -675,6 +675,8 @@ class Categorical(Distribution):
             raise ValueError(
                 "given and logits cannot broadcast to match. ({} vs. {})"
                 .format(tuple(given.shape), tuple(shape)))
+        # (logits that somebody has read are used: log_prob has a gradient
+        # for them; both forms are float32 throughout)
         if self._lazy is not None and self._logits_dense is None and \
                 tuple(batch) == tuple(shape[:-1]) and self._lazy.many_ok():
             return self._lazy.log_prob(given.expand(batch).to(torch.int64))
